@@ -56,6 +56,11 @@ enum {
   H3_OUT_I32 = 3       /* h3_unpack8_finish only: the restored INT32 sum, no dequant    */
 };
 
+/* Element types, norms and position types of the operators around the projections */
+enum { H3_TYPE_F32 = 0, H3_TYPE_F16 = 1, H3_TYPE_BF16 = 2 };
+enum { H3_NORM_NONE = 0, H3_NORM_RMS = 1, H3_NORM_LAYER = 2 };
+enum { H3_POS_I32 = 0, H3_POS_I64 = 1, H3_POS_F32 = 2 };
+
 /* ----------------------------------------------------------------------------
  * Library / device status
  * ------------------------------------------------------------------------- */
@@ -396,6 +401,63 @@ int h3_column_linear_noalloc(const void* x_f16, int64_t m, int64_t k, int convro
                              int64_t weight_scale_len, const float* bias, void* out_f16,
                              void* stream);
 int h3_column_linear_noalloc_error(int device, int* code);
+
+/* ----------------------------------------------------------------------------
+ * Operators of a DiT block around its projections
+ * ------------------------------------------------------------------------- */
+
+/* Residual update joined with the norms before and after it, one pass over the row:
+ *   b  = norm_post(branch),  x' = residual_scale * x + gate[l] * b
+ *   h  = norm_pre(x') * (1 + scale[l]) + shift[l]
+ * l = labels[row] (NULL with mod_rows == 1; a label outside [0, mod_rows) reads row 0
+ * and sets the device error word).  norm: H3_NORM_NONE, _RMS (v * rsqrt(mean v^2 + eps)
+ * * w + b) or _LAYER ((v - mean) * rsqrt(var + eps) * w + b); weight and bias may be
+ * NULL.  gate / shift / scale: fp32 rows of `width` values, *_ld elements apart; NULL
+ * reads as 1, 0 and 0.  x, out and h have x_type (F32, F16 or BF16); branch has it
+ * too, or is F32.  out may be x (each thread writes what it read) and must not
+ * otherwise overlap an input.  Exactly one of h and (q, row_scale) is written when
+ * pre_kind is not NONE: h rounded once to x_type, or the INT8 codes and row scale of h
+ * (rotated by ConvRot256 when convrot; width % 256 == 0 then).  Without a branch (NULL,
+ * out NULL, no gate, no post norm, residual_scale 1) only the pre-norm runs.
+ * width <= 32768; statistics and everything between the two roundings in fp32. */
+int h3_residual_norm(const void* x, int x_type, const void* branch, int branch_type,
+                     int64_t rows, int64_t width, float residual_scale, const float* gate,
+                     int64_t gate_ld, const float* shift, int64_t shift_ld,
+                     const float* scale, int64_t scale_ld, int64_t mod_rows,
+                     const int32_t* labels, int post_kind, const float* post_weight,
+                     const float* post_bias, float post_eps, int pre_kind,
+                     const float* pre_weight, const float* pre_bias, float pre_eps, void* out,
+                     void* h, int convrot, int8_t* q, float* row_scale, void* stream);
+
+/* Per-head RMS norm (norm != 0; weight of head_dim values or NULL) and rotary positions
+ * over several axes, for q and (unless NULL) k:
+ *   v = x * rsqrt(mean(x^2) + eps) * weight,  angle = 2 pi * pos[token][axis[p]] * turns[p]
+ *   (v1, v2) -> (v1 cos - v2 sin, v2 cos + v1 sin)
+ * pair p is (p, p + pairs) when half, else (2p, 2p + 1); elements from 2 * pairs on are
+ * normed and not turned.  Tensors are [tokens][heads][head_dim] of `type` with token and
+ * head strides in elements and unit stride inside a head; an output may be its own
+ * input (same pointer and strides) and must not otherwise overlap an input.  positions:
+ * [tokens][axes] int32, int64 or fp32 (pos_kind).  turns (double) and axis are HOST
+ * arrays of `pairs` entries, copied before the call returns.  head_dim <= 256. */
+int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads,
+                    void* q_out, int64_t qo_token, int64_t qo_head, const void* k,
+                    int64_t k_token, int64_t k_head, int64_t k_heads, void* k_out,
+                    int64_t ko_token, int64_t ko_head, int64_t tokens, int64_t head_dim,
+                    int type, const void* positions, int pos_kind, int axes,
+                    const double* turns, const uint8_t* axis, int64_t pairs, int half, int norm,
+                    const float* q_weight, const float* k_weight, float eps, void* stream);
+
+/* Few rows times a 4-bit weight with group scales:
+ *   y[m][n] = sum_g scales[n][g] * sum_{k in g} x[m][k] (code[n][k] - zero[n][g]) + bias[n]
+ * x: F16 or BF16 rows x_ld elements apart; w: [n][ceil(k / 2)] bytes, code k in the low
+ * nibble of byte k / 2 for even k, in the high one for odd k; scales: [n][ceil(k / group)]
+ * of scale_type; zeros: the same shape in bytes (0 to 15), or NULL for 8 everywhere; bias
+ * may be NULL; out: [m][n] of x_type or F32.  group 32, 64 or 128.  Products of codes and
+ * x are exact; sums are fp32. */
+int h3_int4_linear(const void* x, int x_type, int64_t x_ld, int64_t m, int64_t k,
+                   const uint8_t* w, int64_t n, const void* scales, int scale_type,
+                   const uint8_t* zeros, int group, const float* bias, void* out, int out_type,
+                   void* stream);
 
 /* ----------------------------------------------------------------------------
  * Diagnostics

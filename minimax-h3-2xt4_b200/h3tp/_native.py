@@ -27,11 +27,21 @@ OUT_F32 = 0
 OUT_F16 = 1
 OUT_RESIDUAL = 2
 OUT_I32 = 3
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+NORM_NONE = 0
+NORM_RMS = 1
+NORM_LAYER = 2
+POS_I32 = 0
+POS_I64 = 1
+POS_F32 = 2
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _U32 = ctypes.c_uint32
+_F = ctypes.c_float
 _PP = ctypes.POINTER(ctypes.c_void_p)
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
@@ -79,6 +89,11 @@ SIGNATURES = {
     "h3_peer_gather": [_PP, _I, _I, _I64, _I64, _I64, _I64, _P, _U32, _P],
     "h3_swiglu_rotate_quantize_peer": [_P, _I, _I64, _I64, _PP, _I, _I, _I64, _U32, _I, _P, _P,
                                        _P, _P],
+    "h3_residual_norm": [_P, _I, _P, _I, _I64, _I64, _F, _P, _I64, _P, _I64, _P, _I64, _I64, _P,
+                         _I, _P, _P, _F, _I, _P, _P, _F, _P, _P, _I, _P, _P, _P],
+    "h3_qk_norm_rope": [_P, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64,
+                        _I64, _I64, _I, _P, _I, _I, _P, _P, _I64, _I, _I, _P, _P, _F, _P],
+    "h3_int4_linear": [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I, _P, _I, _P, _P, _I, _P],
     "h3_expf_compare": [_P, _I64, _P, _P, _P],
     "h3_silu_compare": [_P, _I64, _P, _P, _P, _P],
     "h3_quant_compare": [_P, _P, _I64, _P, _P, _P],

@@ -7,6 +7,7 @@ the reference's shapes: activation scales [M, 1] fp32, weight scales [N, 1] fp32
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -482,6 +483,304 @@ def gated_add(residual, branch, gate=None, labels=None):
     N.call("h3_gated_add", b.data_ptr(), kind, M, Nn, res.data_ptr(), _ptr(g), grows, _ptr(lab),
            _stream(b))
     return residual
+
+
+# ----------------------------------------------------------------------------
+# operators of a block around its projections
+# ----------------------------------------------------------------------------
+_TYPES = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
+_NORM_KINDS = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}
+_POSITIONS = {torch.int32: N.POS_I32, torch.int64: N.POS_I64, torch.float32: N.POS_F32}
+
+
+def _inference(where: str, device, **tensors) -> None:
+    """Every tensor on `device`, none that autograd would have to follow."""
+    grad = torch.is_grad_enabled()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name}: on {t.device}, the call runs on {device}")
+        if grad and t.requires_grad:
+            raise ValueError(f"{where} has no backward ({name} requires a gradient): call it under "
+                             "torch.no_grad()")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses [first, last) that a strided tensor's elements lie in."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+class NormSpec(NamedTuple):
+    """A norm over the last dimension: kind 'rms' (v * rsqrt(mean(v^2) + eps)) or 'layer'
+    ((v - mean) * rsqrt(var + eps)), times `weight`, plus `bias` (fp32 [width] or None)."""
+    kind: str = "rms"
+    weight: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+
+
+def _norm_args(spec: Optional[NormSpec], width: int, name: str):
+    if spec is None:
+        return N.NORM_NONE, None, None, 0.0
+    if spec.kind not in _NORM_KINDS:
+        raise ValueError(f"{name}: norm kind must be 'rms' or 'layer'")
+    if not spec.eps >= 0.0:
+        raise ValueError(f"{name}: eps must not be negative")
+    w = None if spec.weight is None else _vec(spec.weight, width, f"{name} weight")
+    b = None if spec.bias is None else _vec(spec.bias, width, f"{name} bias")
+    return _NORM_KINDS[spec.kind], w, b, float(spec.eps)
+
+
+def _table(t, rows, width: int, name: str):
+    """A modulation table [rows, width] with unit stride inside a row (a slice of a wider
+    table is read in place)."""
+    if t is None:
+        return None, 0
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or t.ndim != 2:
+        raise ValueError(f"{name}: fp32 CUDA table [rows, {width}] required")
+    if t.shape[1] != width or t.shape[0] != rows:
+        raise ValueError(f"{name}: table [{rows}, {width}] required, got {tuple(t.shape)}")
+    if t.stride(1) != 1 and width > 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[NormSpec] = None,
+                  pre: Optional[NormSpec] = None, shift=None, scale=None,
+                  residual_scale: float = 1.0, out=None, quantize=False, convrot=True):
+    """Residual update joined with the norms before and after it, one pass over each row:
+
+        b  = post(branch)                                       (post None: the branch itself)
+        x' = residual_scale * x + gate[label] * b
+        h  = pre(x') * (1 + scale[label]) + shift[label]        (pre None: not computed)
+
+    x [M, N] (N <= 32768) is fp32, fp16 or bf16; branch has x's type or fp32.  x' is
+    written over x unless `out` (another [M, N] of x's type) is given, rounded once;
+    without a branch x is left as it is and only `pre` runs.  h comes in x's type or,
+    with quantize, as the INT8 codes and row scales that
+    ColumnParallelLinearINT8.forward_quantized takes (convrot: of the row rotated by
+    ConvRot256, N % 256 == 0).  Statistics, x' and h stay in fp32 until those roundings.
+
+    gate, shift, scale: fp32 tables [R, N], all of the same R (slices of one wider table
+    are read in place); labels: int32 [M], needed unless R is 1.  A label out of range
+    reads row 0 and sets the device error word.
+
+    Returns (x', h or codes or None, row_scale [M, 1] or None)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.ndim != 2 or x.dtype not in _TYPES:
+        raise ValueError("x: 2-D CUDA tensor of fp32, fp16 or bf16 required")
+    if not x.is_contiguous():
+        raise ValueError("x must be contiguous (updated in place)")
+    M, width = x.shape
+    if not 1 <= width <= 32768:
+        raise ValueError("x: a width of 1 to 32768 is required")
+    dev = x.device
+    if pre is None and (quantize or shift is not None or scale is not None):
+        raise ValueError("shift, scale and quantize belong to the pre-norm: give pre")
+    if quantize and convrot and width % 256:
+        raise ValueError("ConvRot256 needs a width that is a multiple of 256")
+    _inference("residual_norm", dev, x=x, branch=branch, gate=gate, labels=labels, shift=shift,
+               scale=scale, out=out)
+    if branch is None:
+        if pre is None or post is not None or gate is not None or out is not None \
+                or residual_scale != 1.0:
+            raise ValueError("without a branch only the pre-norm of x applies")
+        xo = None
+    else:
+        if branch.dtype not in (x.dtype, torch.float32) or branch.shape != x.shape:
+            raise ValueError(f"branch: {tuple(x.shape)} of {x.dtype} or fp32 required")
+        branch = branch.contiguous()
+        xo = x if out is None else _out(out, x.shape, x.dtype, dev, "out")
+        if not _apart(xo, branch) or (xo.data_ptr() != x.data_ptr() and not _apart(xo, x)):
+            raise ValueError("out must be x itself or overlap neither x nor the branch")
+    rows = next((t.shape[0] for t in (gate, shift, scale)
+                 if isinstance(t, torch.Tensor) and t.ndim == 2), 1)
+    g, g_ld = _table(gate, rows, width, "gate")
+    sh, sh_ld = _table(shift, rows, width, "shift")
+    sc, sc_ld = _table(scale, rows, width, "scale")
+    if rows < 1:
+        raise ValueError("the modulation tables must have a row")
+    lab = None
+    if rows > 1 or labels is not None:
+        if labels is None:
+            raise ValueError("labels required for a multi-row modulation table")
+        lab = _need(labels, torch.int32, "labels", 1)
+        if lab.numel() != M:
+            raise ValueError("one label per row required")
+    for spec, name in ((post, "post"), (pre, "pre")):
+        if spec is not None:
+            _inference("residual_norm", dev, **{name + " weight": spec.weight, name + " bias": spec.bias})
+    pk, pw, pb, pe = _norm_args(post, width, "post")
+    nk, nw, nb, ne = _norm_args(pre, width, "pre")
+    h = q = s = None
+    if quantize:
+        q = torch.empty((M, width), dtype=torch.int8, device=dev)
+        s = torch.empty((M, 1), dtype=torch.float32, device=dev)
+    elif pre is not None:
+        h = torch.empty_like(x)
+    if M == 0:
+        return x if xo is None else xo, q if quantize else h, s
+    kind = _TYPES[x.dtype]
+    N.call("h3_residual_norm", x.data_ptr(), kind, _ptr(branch),
+           kind if branch is None else _TYPES[branch.dtype], M, width, float(residual_scale),
+           _ptr(g), g_ld, _ptr(sh), sh_ld, _ptr(sc), sc_ld, rows, _ptr(lab), pk, _ptr(pw), _ptr(pb),
+           pe, nk, _ptr(nw), _ptr(nb), ne, _ptr(xo), _ptr(h), int(bool(convrot)), _ptr(q), _ptr(s),
+           _stream(x))
+    return x if xo is None else xo, q if quantize else h, s
+
+
+def _heads(t, name: str, like=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.ndim != 3 or t.dtype not in _TYPES:
+        raise ValueError(f"{name}: CUDA tensor [tokens, heads, head_dim] of fp32, fp16 or bf16 required")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: unit stride inside a head required")
+    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]
+                             or t.shape[2] != like.shape[2]):
+        raise ValueError(f"{name}: the token count, head_dim and type of q required")
+    return t
+
+
+def _head_windows_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [tokens, heads, dim] views share no element: their spans are apart, or
+    (views of one packed row) their heads lie in disjoint windows of one token stride."""
+    if _apart(a, b):
+        return True
+    period = a.stride(0)
+    if period != b.stride(0) or a.shape[0] < 2 and b.shape[0] < 2:
+        return False
+    wide = [(t.shape[1] - 1) * t.stride(1) + t.shape[2] for t in (a, b)]
+    diff = b.data_ptr() - a.data_ptr()
+    if diff % a.element_size() or min(a.stride(1), b.stride(1)) < 0:
+        return False
+    diff = diff // a.element_size() % period
+    return max(wide) <= period and wide[0] <= diff and diff + wide[1] <= period
+
+
+def _head_out(out, like, name: str):
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    _heads(out, name, like)
+    if out.shape != like.shape:
+        raise ValueError(f"{name}: {tuple(like.shape)} required")
+    # distinct elements at distinct addresses: token-major or head-major
+    (s, h, d), (ts, hs, _) = out.shape, out.stride()
+    if out.numel() and not ((h == 1 or hs >= d) and (s == 1 or ts >= (h - 1) * hs + d)
+                            or (s == 1 or ts >= d) and (h == 1 or hs >= (s - 1) * ts + d)):
+        raise ValueError(f"{name}: overlapping strides")
+    return out
+
+
+def qk_norm_rope(q, k, positions, plan, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+                 norm: bool = True, out_q=None, out_k=None):
+    """Per-head RMS norm and rotary positions of q [S, Hq, D] and k [S, Hk, D] (or None);
+    h3tp.rms_rope documents the arguments.  Returns (q', k')."""
+    _heads(q, "q")
+    dev, (S, hq, D) = q.device, q.shape
+    if D != plan.head_dim:
+        raise ValueError(f"q: head_dim {plan.head_dim} of the plan required, got {D}")
+    if hq < 1 or (k is not None and k.ndim == 3 and k.shape[1] < 1):
+        raise ValueError("at least one head required")
+    if k is not None:
+        _heads(k, "k", q)
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITIONS:
+        raise ValueError("positions: int32, int64 or fp32 tensor required")
+    if positions.ndim == 1 and plan.n_axes == 1:
+        positions = positions.unsqueeze(1)
+    if tuple(positions.shape) != (S, plan.n_axes):
+        raise ValueError(f"positions: [{S}, {plan.n_axes}] required, got {tuple(positions.shape)}")
+    if not eps >= 0.0:
+        raise ValueError("eps must not be negative")
+    if not norm and (q_weight is not None or k_weight is not None):
+        q_weight = k_weight = None
+    _inference("qk_norm_rope", dev, q=q, k=k, positions=positions, q_weight=q_weight,
+               k_weight=k_weight, out_q=out_q, out_k=out_k)
+    positions = positions.contiguous()
+    wq = None if q_weight is None else _vec(q_weight, D, "q_weight")
+    wk = None if k_weight is None or k is None else _vec(k_weight, D, "k_weight")
+    if out_q is not None or out_k is not None:
+        _check_head_outs(q, k, out_q, out_k)
+    oq = _head_out(out_q, q, "out_q")
+    ok = None if k is None else _head_out(out_k, k, "out_k")
+    if S == 0:
+        return oq, ok
+    N.call("h3_qk_norm_rope", q.data_ptr(), q.stride(0), q.stride(1), hq, oq.data_ptr(),
+           oq.stride(0), oq.stride(1), _ptr(k), 0 if k is None else k.stride(0),
+           0 if k is None else k.stride(1), 0 if k is None else k.shape[1], _ptr(ok),
+           0 if k is None else ok.stride(0), 0 if k is None else ok.stride(1), S, D,
+           _TYPES[q.dtype], positions.data_ptr(), _POSITIONS[positions.dtype], plan.n_axes,
+           plan.turns, plan.axis, plan.pairs, plan.half, int(bool(norm)), _ptr(wq), _ptr(wk),
+           float(eps), _stream(q))
+    return oq, ok
+
+
+def _check_head_outs(q, k, out_q, out_k) -> None:
+    """Outputs that are given must be their own input, or share no element with an input
+    or with each other."""
+    if out_k is not None and k is None:
+        raise ValueError("out_k without k")
+    for out, own, other, name in ((out_q, q, k, "out_q"), (out_k, k, q, "out_k")):
+        if out is None:
+            continue
+        _head_out(out, own, name)
+        same = out.data_ptr() == own.data_ptr() and out.stride() == own.stride()
+        if not same and not _head_windows_apart(out, own):
+            raise ValueError(f"{name} must be its input or not overlap it")
+        if other is not None and not _head_windows_apart(out, other):
+            raise ValueError(f"{name} overlaps the other input")
+    if out_q is not None and out_k is not None and not _head_windows_apart(out_q, out_k):
+        raise ValueError("out_q and out_k overlap")
+
+
+INT4_GROUPS = (32, 64, 128)
+
+
+def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, out_dtype=None):
+    """y = x @ W.T + bias with W[n, k] = scales[n, k // group] * (code[n, k] - zero), codes of
+    4 bits; x fp16 or bf16 [M, K], y [M, N] in x's type or fp32 (out_dtype).
+
+    weight: contiguous uint8 [N, ceil(K / 2)], code k in the low nibble of byte k // 2 for
+    even k and in the high one for odd k; scales: fp32, fp16 or bf16 [N, ceil(K / group)];
+    zeros: uint8 of the same shape (0 to 15), None for 8 everywhere; bias: fp32 [N].
+    Meant for few rows (a token or a handful): the weight is read once for every 32 rows."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.ndim != 2 \
+            or x.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError("x: 2-D CUDA tensor of fp16 or bf16 required")
+    M, K = x.shape
+    if group not in INT4_GROUPS:
+        raise ValueError(f"group must be one of {INT4_GROUPS}")
+    if weight.dtype != torch.uint8 or weight.ndim != 2 or not weight.is_contiguous() or K < 1 \
+            or weight.shape[0] < 1 or weight.shape[1] != (K + 1) // 2:
+        raise ValueError(f"weight: contiguous uint8 [N, {(K + 1) // 2}] required")
+    n = weight.shape[0]
+    shape = (n, -(-K // group))
+    if scales.dtype not in _TYPES or tuple(scales.shape) != shape:
+        raise ValueError(f"scales: {shape} of fp32, fp16 or bf16 required")
+    if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
+        raise ValueError(f"zeros: uint8 {shape} required")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in (x.dtype, torch.float32):
+        raise ValueError("out_dtype must be x's type or fp32")
+    _inference("int4_linear", x.device, x=x, weight=weight, scales=scales, zeros=zeros, bias=bias)
+    if K > 1 and x.stride(1) != 1 or x.stride(0) < K:
+        x = x.contiguous()
+    scales = scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    b = None if bias is None else _vec(bias, n, "bias")
+    out = torch.empty((M, n), dtype=out_dtype, device=x.device)
+    if M == 0:
+        return out
+    N.call("h3_int4_linear", x.data_ptr(), _TYPES[x.dtype], x.stride(0) if M > 1 else K, M, K,
+           weight.data_ptr(), n, scales.data_ptr(), _TYPES[scales.dtype], _ptr(zeros), group,
+           _ptr(b), out.data_ptr(), _TYPES[out_dtype], _stream(x))
+    return out
 
 
 def peer_reduce(bases, world: int, rank: int, flags_off: int, partial_off: int, final_off: int,
