@@ -1,11 +1,21 @@
 // Per-head RMS norm and rotary positions over several axes, on the q and k heads of a
 // projection's output.  Pair p of a head turns by pos[token][axis[p]] * frequency[p]:
 //   (v1, v2) <- (v1 cos - v2 sin, v2 cos + v1 sin)
+//
+// Bound by HBM: every element is read and written once, and the sines and cosines are
+// computed in the kernel (a table of them would be read and written too).  They depend on
+// the token and the pair alone, so a CTA takes all heads of a few tokens: it computes the
+// angles of its tokens once into shared memory and then streams their heads past them.
+// A head is held by G = 8, 16 or 32 lanes, eight elements (four pairs) each, one 16-byte
+// load or two of 8 bytes; the sum of squares is a shuffle tree over those lanes.
 #include "h3_types.cuh"
 
 namespace h3 {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
+constexpr int kRopeThreads = 256;
+constexpr int kRopeTokens = 8;   // most tokens of one CTA tile
+constexpr int kRopeAhead = 4;    // heads a lane group has in flight
 
 struct HeadView {
   const void* in;
@@ -20,7 +30,9 @@ struct HeadView {
 struct RopeArgs {
   HeadView q, k;
   int64_t tokens;
-  int dim, pairs, axes, pos_kind, half, norm;
+  int dim, pairs, axes, pos_kind, norm;
+  int tile_tokens, tile_heads;  // of one CTA
+  uint32_t head_magic;          // ceil(2^32 / tile_heads)
   float eps, inv_dim;
   const void* positions;
   double turns[kMaxPairs];      // frequency / (2 pi)
@@ -29,59 +41,221 @@ struct RopeArgs {
 
 // Angles of far positions need more than 24 bits: the turns are reduced to a fraction of
 // one in 64 bits, and the sine and cosine of that fraction taken in 32.
-H3_DEV void pair_angle(const RopeArgs& a, int64_t token, int p, float& c, float& s) {
+H3_DEV float2 pair_angle(const RopeArgs& a, int64_t token, int p) {
   const int64_t at = token * a.axes + a.axis[p];
   double pos;
   if (a.pos_kind == H3_POS_I32) pos = (double)__ldg(reinterpret_cast<const int32_t*>(a.positions) + at);
-  else if (a.pos_kind == H3_POS_I64) pos = (double)reinterpret_cast<const int64_t*>(a.positions)[at];
+  else if (a.pos_kind == H3_POS_I64) pos = (double)__ldg(reinterpret_cast<const long long*>(a.positions) + at);
   else pos = (double)__ldg(reinterpret_cast<const float*>(a.positions) + at);
   const double t = pos * a.turns[p];
+  float s, c;
   sincospif(2.0f * (float)(t - rint(t)), &s, &c);
+  return make_float2(c, s);
+}
+
+// The four pairs of a lane: first elements in v[0..3], second in v[4..7] when the pairs
+// are halves apart, (v[2i], v[2i + 1]) otherwise.  VEC: whole 16-byte (or 8-byte) pieces;
+// else one element at a time, any alignment and any head_dim.
+template <typename T, bool HALF, bool VEC>
+struct HeadLane {
+  Raw<T, 8> r;        // VEC
+  float x[8];         // !VEC
+
+  H3_DEV static int element(const RopeArgs& a, int u, int i) {
+    if (!HALF) return 8 * u + i;
+    const int p = 4 * u + (i & 3);          // pair p's element i / 4
+    if (p < a.pairs) return i < 4 ? p : p + a.pairs;
+    return 2 * p + (i >> 2);                // behind the turned elements: neighbours
+  }
+  H3_DEV void load(const RopeArgs& a, const T* p, int u) {
+    if constexpr (VEC) {
+      if (HALF && 4 * u < a.pairs) {
+        Raw<T, 4> lo, hi;
+        lo.load(p + 4 * u);
+        hi.load(p + a.pairs + 4 * u);
+#pragma unroll
+        for (int i = 0; i < Raw<T, 4>::kWords; ++i) {
+          r.w[i] = lo.w[i];
+          r.w[Raw<T, 4>::kWords + i] = hi.w[i];
+        }
+      } else {
+        r.load(p + 8 * u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = element(a, u, i);
+        x[i] = e < a.dim ? to_f32(p[e]) : 0.0f;
+      }
+    }
+  }
+  H3_DEV void values(float* v) const {
+    if constexpr (VEC) {
+      r.unpack(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = x[i];
+    }
+  }
+  H3_DEV static void store(const RopeArgs& a, T* p, int u, const float* v) {
+    if constexpr (VEC) {
+      if (HALF && 4 * u < a.pairs) {
+        Raw<T, 4> lo, hi;
+        lo.pack(v);
+        hi.pack(v + 4);
+        lo.store(p + 4 * u);
+        hi.store(p + a.pairs + 4 * u);
+      } else {
+        Raw<T, 8> o;
+        o.pack(v);
+        o.store(p + 8 * u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = element(a, u, i);
+        if (e < a.dim) p[e] = from_f32<T>(v[i]);
+      }
+    }
+  }
+  // weight of element i of this lane; VEC keeps neighbours behind the turned elements in
+  // memory order, so there the index is the memory's
+  H3_DEV static int weight_index(const RopeArgs& a, int u, int i) {
+    if (VEC && HALF && 4 * u >= a.pairs) return 8 * u + i;
+    return element(a, u, i);
+  }
+};
+
+template <typename T, bool HALF, bool VEC, int G>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
+  __shared__ __align__(16) float2 turn[kRopeTokens][kMaxPairs];
+  constexpr int kGroups = kRopeThreads / G;
+  using Lane = HeadLane<T, HALF, VEC>;
+  const int u = threadIdx.x % G, group = threadIdx.x / G;
+  const int64_t token0 = (int64_t)blockIdx.x * a.tile_tokens;
+  const int tokens = (int)min((int64_t)a.tile_tokens, a.tokens - token0);
+  const int head0 = blockIdx.y * a.tile_heads;
+  const int heads = min(a.tile_heads, a.q.heads + a.k.heads - head0);
+  const int items = tokens * a.tile_heads;
+  const bool live = 8 * u < a.dim;
+
+  // the angles of the tile; pairs behind the turned ones are never read
+  const int turns = tokens * a.pairs;
+  for (int i = threadIdx.x; i < turns; i += kRopeThreads) {
+    const int t = i / a.pairs, p = i - t * a.pairs;
+    turn[t][p] = pair_angle(a, token0 + t, p);
+  }
+  float wq[8], wk[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = Lane::weight_index(a, u, i);
+    wq[i] = a.q.weight != nullptr && e < a.dim ? __ldg(a.q.weight + e) : 1.0f;
+    wk[i] = a.k.weight != nullptr && e < a.dim ? __ldg(a.k.weight + e) : 1.0f;
+  }
+  __syncthreads();
+
+  // every lane of the CTA makes every step (the shuffles need them all); `head` is -1
+  // where there is nothing to do
+  for (int base = group; base - group < items; base += kGroups * kRopeAhead) {
+    Lane lane[kRopeAhead];
+    int tok[kRopeAhead], head[kRopeAhead];
+#pragma unroll
+    for (int j = 0; j < kRopeAhead; ++j) {
+      const int it = base + j * kGroups;
+      // it / tile_heads: exact, their product is below 2^32; 2^32 itself has no 32-bit form
+      tok[j] = a.head_magic != 0 ? (int)__umulhi((uint32_t)it, a.head_magic) : it;
+      head[j] = it - tok[j] * a.tile_heads;
+      head[j] = it < items && head[j] < heads && live ? head[j] + head0 : -1;
+      if (head[j] >= 0) {
+        const bool is_k = head[j] >= a.q.heads;
+        const T* in = reinterpret_cast<const T*>(is_k ? a.k.in : a.q.in);
+        in += (token0 + tok[j]) * (is_k ? a.k.in_token : a.q.in_token) +
+              (is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.in_head : a.q.in_head);
+        lane[j].load(a, in, u);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRopeAhead; ++j) {
+      float v[8];
+      const bool is_k = head[j] >= a.q.heads;
+      if (head[j] >= 0) {
+        lane[j].values(v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      }
+      if (a.norm) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __fmaf_rn(v[i], v[i], sum);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = rsqrtf(__fmaf_rn(sum, a.inv_dim, a.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (is_k ? wk[i] : wq[i]);
+      }
+      if (head[j] < 0) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (4 * u + i >= a.pairs) continue;
+        const float2 cs = turn[tok[j]][4 * u + i];
+        float& v1 = v[HALF ? i : 2 * i];
+        float& v2 = v[HALF ? i + 4 : 2 * i + 1];
+        const float r1 = __fmaf_rn(v1, cs.x, -(v2 * cs.y));
+        v2 = __fmaf_rn(v2, cs.x, v1 * cs.y);
+        v1 = r1;
+      }
+      T* out = reinterpret_cast<T*>(is_k ? a.k.out : a.q.out);
+      out += (token0 + tok[j]) * (is_k ? a.k.out_token : a.q.out_token) +
+             (is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.out_head : a.q.out_head);
+      Lane::store(a, out, u, v);
+    }
+  }
+}
+
+template <typename T, bool HALF, bool VEC, int G>
+int launch_rope(RopeArgs& a, int sms, cudaStream_t stream) {
+  // A tile is the smallest number of tokens whose heads fill the lane groups kRopeAhead
+  // times; with too few tiles for the SMs it shrinks, at last to a part of one token's
+  // heads (one round of the lane groups).
+  constexpr int kGroups = kRopeThreads / G;
+  const int heads = a.q.heads + a.k.heads;
+  int tokens = std::min<int>((kGroups * kRopeAhead + heads - 1) / heads, kRopeTokens);
+  while (tokens > 1 && (a.tokens + tokens - 1) / tokens < sms) tokens /= 2;
+  a.tile_tokens = tokens;
+  a.tile_heads = heads;
+  const int64_t tiles = (a.tokens + tokens - 1) / tokens;
+  if (tokens == 1 && tiles < sms)
+    a.tile_heads = std::min<int>(heads, kGroups * std::max<int>(1, (int)(tiles * heads / ((int64_t)sms * kGroups))));
+  const int splits = (heads + a.tile_heads - 1) / a.tile_heads;
+  a.head_magic = (uint32_t)(((1ull << 32) + a.tile_heads - 1) / a.tile_heads);
+  if (tiles > 0x7fffffff || splits > 65535) return H3_ERR_INVALID;
+  rope_kernel<T, HALF, VEC, G><<<dim3((unsigned)tiles, (unsigned)splits), kRopeThreads, 0, stream>>>(a);
+  return h3host::check_launch();
+}
+
+template <typename T, bool HALF, bool VEC>
+int launch_rope_width(RopeArgs& a, int sms, cudaStream_t stream) {
+  if (a.dim <= 64) return launch_rope<T, HALF, VEC, 8>(a, sms, stream);
+  if (a.dim <= 128) return launch_rope<T, HALF, VEC, 16>(a, sms, stream);
+  return launch_rope<T, HALF, VEC, 32>(a, sms, stream);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) rope_kernel(const __grid_constant__ RopeArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int heads = a.q.heads + a.k.heads;
-  const int64_t items = a.tokens * heads;
-  for (int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < items; i += gridDim.x * 8ll) {
-    const int64_t token = i / heads;
-    int head = (int)(i - token * heads);
-    const bool is_k = head >= a.q.heads;
-    const HeadView& v = is_k ? a.k : a.q;
-    if (is_k) head -= a.q.heads;
-    const T* in = reinterpret_cast<const T*>(v.in) + token * v.in_token + head * v.in_head;
-    T* out = reinterpret_cast<T*>(v.out) + token * v.out_token + head * v.out_head;
-    float x[8];
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = lane + 32 * j;
-      x[j] = c < a.dim ? to_f32(in[c]) : 0.0f;
-      sum = __fmaf_rn(x[j], x[j], sum);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float inv = a.norm ? __frsqrt_rn(__fmaf_rn(sum, a.inv_dim, a.eps)) : 1.0f;
-    __shared__ float row[8][256];
-    float* w = row[threadIdx.x >> 5];
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = lane + 32 * j;
-      if (c < a.dim) w[c] = x[j] * inv * (a.norm && v.weight != nullptr ? __ldg(v.weight + c) : 1.0f);
-    }
-    __syncwarp();
-    for (int p = lane; p < a.pairs; p += 32) {
-      float cs, sn;
-      pair_angle(a, token, p, cs, sn);
-      const int c1 = a.half ? p : 2 * p, c2 = a.half ? p + a.pairs : 2 * p + 1;
-      const float v1 = w[c1], v2 = w[c2];
-      out[c1] = from_f32<T>(__fmaf_rn(v1, cs, -(v2 * sn)));
-      out[c2] = from_f32<T>(__fmaf_rn(v2, cs, v1 * sn));
-    }
-    for (int c = 2 * a.pairs + lane; c < a.dim; c += 32) out[c] = from_f32<T>(w[c]);
+int launch_rope_type(RopeArgs& a, bool half, int sms, cudaStream_t stream) {
+  // whole 16-byte pieces: every head starts on a 16-byte boundary, is a multiple of eight
+  // elements, and halves (if paired so) are multiples of four pairs
+  bool vec = a.dim % 8 == 0 && (!half || a.pairs % 4 == 0);
+  for (const HeadView* v : {&a.q, &a.k}) {
+    if (v->heads == 0) continue;
+    vec = vec && h3host::aligned(v->in, 16) && h3host::aligned(v->out, 16);
+    for (int64_t s : {v->in_token, v->in_head, v->out_token, v->out_head})
+      vec = vec && s * (int64_t)sizeof(T) % 16 == 0;
   }
+  if (half) return vec ? launch_rope_width<T, true, true>(a, sms, stream)
+                       : launch_rope_width<T, true, false>(a, sms, stream);
+  return vec ? launch_rope_width<T, false, true>(a, sms, stream)
+             : launch_rope_width<T, false, false>(a, sms, stream);
 }
 
 }  // namespace h3
@@ -97,10 +271,10 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
   using namespace h3;
   if (k == nullptr) k_heads = 0;
   if (q == nullptr || q_out == nullptr || (k != nullptr && k_out == nullptr) || tokens < 0 ||
-      q_heads < 1 || q_heads > 65536 || k_heads < 0 || k_heads > 65536 || head_dim < 2 ||
+      q_heads < 1 || q_heads > 4096 || k_heads < 0 || k_heads > 4096 || head_dim < 2 ||
       head_dim > 2 * kMaxPairs || positions == nullptr || axes < 1 || axes > 255 ||
       turns == nullptr || axis == nullptr || pairs < 1 || 2 * pairs > head_dim ||
-      pos_kind < H3_POS_I32 || pos_kind > H3_POS_F32)
+      pos_kind < H3_POS_I32 || pos_kind > H3_POS_F32 || type < H3_TYPE_F32 || type > H3_TYPE_BF16)
     return H3_ERR_INVALID;
   RopeArgs a;
   a.q = HeadView{q, q_out, q_token, q_head, qo_token, qo_head, (int)q_heads, q_weight};
@@ -110,7 +284,6 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
   a.pairs = (int)pairs;
   a.axes = axes;
   a.pos_kind = pos_kind;
-  a.half = half != 0;
   a.norm = norm != 0;
   a.eps = eps;
   a.inv_dim = (float)(1.0 / (double)head_dim);
@@ -125,11 +298,8 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
   h3host::DeviceScope scope;
   if (int s = scope.bind(q, &dev)) return s;
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t ctas = (tokens * (q_heads + k_heads) + 7) / 8;
-  const int grid = (int)std::min<int64_t>(ctas, (int64_t)h3host::sm_count(dev) * 8);
-  if (type == H3_TYPE_F32) rope_kernel<float><<<grid, 256, 0, st>>>(a);
-  else if (type == H3_TYPE_F16) rope_kernel<__half><<<grid, 256, 0, st>>>(a);
-  else if (type == H3_TYPE_BF16) rope_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  else return H3_ERR_INVALID;
-  return h3host::check_launch();
+  const int sms = h3host::sm_count(dev);
+  if (type == H3_TYPE_F32) return launch_rope_type<float>(a, half != 0, sms, st);
+  if (type == H3_TYPE_F16) return launch_rope_type<__half>(a, half != 0, sms, st);
+  return launch_rope_type<__nv_bfloat16>(a, half != 0, sms, st);
 }
