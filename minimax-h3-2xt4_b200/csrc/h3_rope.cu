@@ -4,23 +4,22 @@
 //
 // Bound by HBM: every element is read and written once, and the sines and cosines are
 // computed in the kernel (a table of them would be read and written too).  They depend on
-// the token and the pair alone, so a CTA takes all heads of a few tokens: it computes the
-// angles of its tokens once into shared memory and then streams their heads past them.
-// A head is held by G = 8, 16 or 32 lanes, eight elements (four pairs) each, one 16-byte
-// load or two of 8 bytes; the sum of squares is a shuffle tree over those lanes.
+// the token and the pair alone, so a tile is all heads of a few tokens: a CTA computes the
+// angles of the tile once into shared memory, one pair a thread, and then streams the
+// tile's heads past them.  CTAs are persistent, so that a thread looks its pair's frequency
+// up once.  A head is held by G = 8, 16 or 32 lanes, eight elements (four pairs) each, one
+// 16-byte load or two of 8 bytes; the sum of squares is a shuffle tree over those lanes.
 #include "h3_types.cuh"
 
 namespace h3 {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 constexpr int kRopeThreads = 256;
-constexpr int kRopeTokens = 8;   // most tokens of one CTA tile
-constexpr int kRopeAhead = 4;    // heads a lane group has in flight
 
 struct HeadView {
   const void* in;
   void* out;
-  int64_t in_token, in_head, out_token, out_head;  // strides in elements
+  int in_token, in_head, out_token, out_head;  // strides in elements
   int heads;
   const float* weight;
 };
@@ -41,13 +40,13 @@ struct RopeArgs {
 
 // Angles of far positions need more than 24 bits: the turns are reduced to a fraction of
 // one in 64 bits, and the sine and cosine of that fraction taken in 32.
-H3_DEV float2 pair_angle(const RopeArgs& a, int64_t token, int p) {
-  const int64_t at = token * a.axes + a.axis[p];
+H3_DEV float2 pair_angle(const RopeArgs& a, int64_t token, int axis, double turns) {
+  const int64_t at = token * a.axes + axis;
   double pos;
   if (a.pos_kind == H3_POS_I32) pos = (double)__ldg(reinterpret_cast<const int32_t*>(a.positions) + at);
   else if (a.pos_kind == H3_POS_I64) pos = (double)__ldg(reinterpret_cast<const long long*>(a.positions) + at);
   else pos = (double)__ldg(reinterpret_cast<const float*>(a.positions) + at);
-  const double t = pos * a.turns[p];
+  const double t = pos * turns;
   float s, c;
   sincospif(2.0f * (float)(t - rint(t)), &s, &c);
   return make_float2(c, s);
@@ -127,101 +126,131 @@ struct HeadLane {
 };
 
 template <typename T, bool HALF, bool VEC, int G>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const __grid_constant__ RopeArgs a) {
-  __shared__ __align__(16) float2 turn[kRopeTokens][kMaxPairs];
+__global__ void __launch_bounds__(kRopeThreads, VEC ? 4 : 2)
+    rope_kernel(const __grid_constant__ RopeArgs a) {
+  // A lane reads its four angles and its eight weights as 16-byte words, the lanes of a
+  // group side by side: [buffer][token][pair & 2][lane] and [q, k][half][lane].
+  __shared__ __align__(16) float4 turn[2][kRopeThreads / 2 + 64];
+  __shared__ __align__(16) float4 weight[2][2][32];
   constexpr int kGroups = kRopeThreads / G;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;  // heads a lane group has in flight, 64 bytes a lane
   using Lane = HeadLane<T, HALF, VEC>;
   const int u = threadIdx.x % G, group = threadIdx.x / G;
-  const int64_t token0 = (int64_t)blockIdx.x * a.tile_tokens;
-  const int tokens = (int)min((int64_t)a.tile_tokens, a.tokens - token0);
+  const int quads = (a.pairs + 3) / 4;  // lanes with turned pairs
   const int head0 = blockIdx.y * a.tile_heads;
   const int heads = min(a.tile_heads, a.q.heads + a.k.heads - head0);
-  const int items = tokens * a.tile_heads;
   const bool live = 8 * u < a.dim;
 
-  // the angles of the tile; pairs behind the turned ones are never read
-  const int turns = tokens * a.pairs;
-  for (int i = threadIdx.x; i < turns; i += kRopeThreads) {
-    const int t = i / a.pairs, p = i - t * a.pairs;
-    turn[t][p] = pair_angle(a, token0 + t, p);
-  }
-  float wq[8], wk[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = Lane::weight_index(a, u, i);
-    wq[i] = a.q.weight != nullptr && e < a.dim ? __ldg(a.q.weight + e) : 1.0f;
-    wk[i] = a.k.weight != nullptr && e < a.dim ? __ldg(a.k.weight + e) : 1.0f;
-  }
-  __syncthreads();
-
-  // every lane of the CTA makes every step (the shuffles need them all); `head` is -1
-  // where there is nothing to do
-  for (int base = group; base - group < items; base += kGroups * kRopeAhead) {
-    Lane lane[kRopeAhead];
-    int tok[kRopeAhead], head[kRopeAhead];
-#pragma unroll
-    for (int j = 0; j < kRopeAhead; ++j) {
-      const int it = base + j * kGroups;
-      // it / tile_heads: exact, their product is below 2^32; 2^32 itself has no 32-bit form
-      tok[j] = a.head_magic != 0 ? (int)__umulhi((uint32_t)it, a.head_magic) : it;
-      head[j] = it - tok[j] * a.tile_heads;
-      head[j] = it < items && head[j] < heads && live ? head[j] + head0 : -1;
-      if (head[j] >= 0) {
-        const bool is_k = head[j] >= a.q.heads;
-        const T* in = reinterpret_cast<const T*>(is_k ? a.k.in : a.q.in);
-        in += (token0 + tok[j]) * (is_k ? a.k.in_token : a.q.in_token) +
-              (is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.in_head : a.q.in_head);
-        lane[j].load(a, in, u);
-      }
+  const bool weighted = a.norm && (a.q.weight != nullptr || a.k.weight != nullptr);
+  if (weighted) {
+    for (int i = threadIdx.x; i < 512; i += kRopeThreads) {
+      const float* w = i < 256 ? a.q.weight : a.k.weight;
+      const int lane = (i & 255) >> 3, e = Lane::weight_index(a, lane, i & 7);
+      reinterpret_cast<float*>(&weight[i >> 8][(i >> 2) & 1][lane])[i & 3] =
+          w != nullptr && e < a.dim ? __ldg(w + e) : 1.0f;
     }
+  }
+  // this thread's pair of the tile's angles
+  const int my_tok = threadIdx.x / a.pairs, my_pair = threadIdx.x - my_tok * a.pairs;
+  const double my_turns = my_tok < a.tile_tokens ? a.turns[my_pair] : 0.0;
+  const int my_axis = my_tok < a.tile_tokens ? a.axis[my_pair] : 0;
+  float2* my_slot = reinterpret_cast<float2*>(
+      &turn[0][(my_tok * 2 + ((my_pair >> 1) & 1)) * quads + (my_pair >> 2)]) + (my_pair & 1);
+
+  int buffer = 0;
+  for (int64_t tile = blockIdx.x; tile * a.tile_tokens < a.tokens; tile += gridDim.x, buffer ^= 1) {
+    const int64_t token0 = tile * a.tile_tokens;
+    const int tokens = (int)min((int64_t)a.tile_tokens, a.tokens - token0);
+    const int items = tokens * a.tile_heads;
+    if (my_tok < tokens)
+      my_slot[buffer * (sizeof(turn[0]) / sizeof(float2))] =
+          pair_angle(a, token0 + my_tok, my_axis, my_turns);
+    // one barrier a tile: the buffer written next was last read before this one
+    __syncthreads();
+    const T* q_in = reinterpret_cast<const T*>(a.q.in) + token0 * a.q.in_token;
+    const T* k_in = reinterpret_cast<const T*>(a.k.in) + token0 * a.k.in_token;
+    T* q_out = reinterpret_cast<T*>(a.q.out) + token0 * a.q.out_token;
+    T* k_out = reinterpret_cast<T*>(a.k.out) + token0 * a.k.out_token;
+
+    // every lane of the CTA makes every step (the shuffles need them all); `head` is -1
+    // where there is nothing to do
+    for (int base = group; base - group < items; base += kGroups * kAhead) {
+      Lane lane[kAhead];
+      int tok[kAhead], head[kAhead];
 #pragma unroll
-    for (int j = 0; j < kRopeAhead; ++j) {
-      float v[8];
-      const bool is_k = head[j] >= a.q.heads;
-      if (head[j] >= 0) {
-        lane[j].values(v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int j = 0; j < kAhead; ++j) {
+        const int it = base + j * kGroups;
+        // it / tile_heads: exact, their product is below 2^32; 2^32 itself has no 32-bit form
+        tok[j] = a.head_magic != 0 ? (int)__umulhi((uint32_t)it, a.head_magic) : it;
+        head[j] = it - tok[j] * a.tile_heads;
+        head[j] = it < items && head[j] < heads && live ? head[j] + head0 : -1;
+        if (head[j] >= 0) {
+          const bool is_k = head[j] >= a.q.heads;
+          const T* in = is_k ? k_in : q_in;
+          in += (int64_t)tok[j] * (is_k ? a.k.in_token : a.q.in_token) +
+                (int64_t)(is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.in_head : a.q.in_head);
+          lane[j].load(a, in, u);
+        }
       }
-      if (a.norm) {
-        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __fmaf_rn(v[i], v[i], sum);
+      for (int j = 0; j < kAhead; ++j) {
+        float v[8];
+        const bool is_k = head[j] >= a.q.heads;
+        if (head[j] >= 0) {
+          lane[j].values(v);
+        } else {
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(__fmaf_rn(sum, a.inv_dim, a.eps));
+          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        }
+        if (a.norm) {
+          float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (is_k ? wk[i] : wq[i]);
+          for (int i = 0; i < 8; ++i) sum = __fmaf_rn(v[i], v[i], sum);
+#pragma unroll
+          for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float inv = rsqrtf(__fmaf_rn(sum, a.inv_dim, a.eps));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= inv;
+          if (weighted) {
+            const float4 w0 = weight[is_k][0][u], w1 = weight[is_k][1][u];
+            v[0] *= w0.x; v[1] *= w0.y; v[2] *= w0.z; v[3] *= w0.w;
+            v[4] *= w1.x; v[5] *= w1.y; v[6] *= w1.z; v[7] *= w1.w;
+          }
+        }
+        if (head[j] < 0) continue;
+        if (u < quads) {
+          const float4* t = &turn[buffer][tok[j] * 2 * quads + u];
+          const float4 t0 = t[0], t1 = t[quads];
+          const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (!VEC && 4 * u + i >= a.pairs) continue;
+            if (VEC && !HALF && 4 * u + i >= a.pairs) continue;
+            float& v1 = v[HALF ? i : 2 * i];
+            float& v2 = v[HALF ? i + 4 : 2 * i + 1];
+            const float r1 = __fmaf_rn(v1, c[i], -(v2 * s[i]));
+            v2 = __fmaf_rn(v2, c[i], v1 * s[i]);
+            v1 = r1;
+          }
+        }
+        T* out = is_k ? k_out : q_out;
+        out += (int64_t)tok[j] * (is_k ? a.k.out_token : a.q.out_token) +
+               (int64_t)(is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.out_head : a.q.out_head);
+        Lane::store(a, out, u, v);
       }
-      if (head[j] < 0) continue;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (4 * u + i >= a.pairs) continue;
-        const float2 cs = turn[tok[j]][4 * u + i];
-        float& v1 = v[HALF ? i : 2 * i];
-        float& v2 = v[HALF ? i + 4 : 2 * i + 1];
-        const float r1 = __fmaf_rn(v1, cs.x, -(v2 * cs.y));
-        v2 = __fmaf_rn(v2, cs.x, v1 * cs.y);
-        v1 = r1;
-      }
-      T* out = reinterpret_cast<T*>(is_k ? a.k.out : a.q.out);
-      out += (token0 + tok[j]) * (is_k ? a.k.out_token : a.q.out_token) +
-             (is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.out_head : a.q.out_head);
-      Lane::store(a, out, u, v);
     }
   }
 }
 
 template <typename T, bool HALF, bool VEC, int G>
 int launch_rope(RopeArgs& a, int sms, cudaStream_t stream) {
-  // A tile is the smallest number of tokens whose heads fill the lane groups kRopeAhead
-  // times; with too few tiles for the SMs it shrinks, at last to a part of one token's
-  // heads (one round of the lane groups).
+  // A tile is as many tokens as give every thread one angle; with too few tiles for the
+  // SMs it shrinks, at last to a part of one token's heads (rounds of the lane groups).
   constexpr int kGroups = kRopeThreads / G;
   const int heads = a.q.heads + a.k.heads;
-  int tokens = std::min<int>((kGroups * kRopeAhead + heads - 1) / heads, kRopeTokens);
-  while (tokens > 1 && (a.tokens + tokens - 1) / tokens < sms) tokens /= 2;
+  int tokens = std::max<int>(1, kRopeThreads / a.pairs);
+  tokens = std::min<int>(tokens, 16);
+  while (tokens > 1 && (a.tokens + tokens - 1) / tokens < 2 * sms) tokens /= 2;
   a.tile_tokens = tokens;
   a.tile_heads = heads;
   const int64_t tiles = (a.tokens + tokens - 1) / tokens;
@@ -229,8 +258,8 @@ int launch_rope(RopeArgs& a, int sms, cudaStream_t stream) {
     a.tile_heads = std::min<int>(heads, kGroups * std::max<int>(1, (int)(tiles * heads / ((int64_t)sms * kGroups))));
   const int splits = (heads + a.tile_heads - 1) / a.tile_heads;
   a.head_magic = (uint32_t)(((1ull << 32) + a.tile_heads - 1) / a.tile_heads);
-  if (tiles > 0x7fffffff || splits > 65535) return H3_ERR_INVALID;
-  rope_kernel<T, HALF, VEC, G><<<dim3((unsigned)tiles, (unsigned)splits), kRopeThreads, 0, stream>>>(a);
+  const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * (VEC ? 4 : 2));
+  rope_kernel<T, HALF, VEC, G><<<dim3(grid, splits), kRopeThreads, 0, stream>>>(a);
   return h3host::check_launch();
 }
 
@@ -249,8 +278,8 @@ int launch_rope_type(RopeArgs& a, bool half, int sms, cudaStream_t stream) {
   for (const HeadView* v : {&a.q, &a.k}) {
     if (v->heads == 0) continue;
     vec = vec && h3host::aligned(v->in, 16) && h3host::aligned(v->out, 16);
-    for (int64_t s : {v->in_token, v->in_head, v->out_token, v->out_head})
-      vec = vec && s * (int64_t)sizeof(T) % 16 == 0;
+    for (int s : {v->in_token, v->in_head, v->out_token, v->out_head})
+      vec = vec && (int64_t)s * (int64_t)sizeof(T) % 16 == 0;
   }
   if (half) return vec ? launch_rope_width<T, true, true>(a, sms, stream)
                        : launch_rope_width<T, true, false>(a, sms, stream);
@@ -276,9 +305,12 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
       turns == nullptr || axis == nullptr || pairs < 1 || 2 * pairs > head_dim ||
       pos_kind < H3_POS_I32 || pos_kind > H3_POS_F32 || type < H3_TYPE_F32 || type > H3_TYPE_BF16)
     return H3_ERR_INVALID;
+  if (k == nullptr) k_token = k_head = ko_token = ko_head = 0;
+  for (int64_t s : {q_token, q_head, qo_token, qo_head, k_token, k_head, ko_token, ko_head})
+    if (s < 0 || s > 0x7fffffff) return H3_ERR_INVALID;
   RopeArgs a;
-  a.q = HeadView{q, q_out, q_token, q_head, qo_token, qo_head, (int)q_heads, q_weight};
-  a.k = HeadView{k, k_out, k_token, k_head, ko_token, ko_head, (int)k_heads, k_weight};
+  a.q = HeadView{q, q_out, (int)q_token, (int)q_head, (int)qo_token, (int)qo_head, (int)q_heads, q_weight};
+  a.k = HeadView{k, k_out, (int)k_token, (int)k_head, (int)ko_token, (int)ko_head, (int)k_heads, k_weight};
   a.tokens = tokens;
   a.dim = (int)head_dim;
   a.pairs = (int)pairs;
