@@ -4,17 +4,24 @@
 //
 // Bound by HBM: every element is read and written once, and the sines and cosines are
 // computed in the kernel (a table of them would be read and written too).  They depend on
-// the token and the pair alone, so a tile is all heads of a few tokens: a CTA computes the
-// angles of the tile once into shared memory, one pair a thread, and then streams the
-// tile's heads past them.  CTAs are persistent, so that a thread looks its pair's frequency
-// up once.  A head is held by G = 8, 16 or 32 lanes, eight elements (four pairs) each, one
-// 16-byte load or two of 8 bytes; the sum of squares is a shuffle tree over those lanes.
+// the token and the pair alone, so a lane group takes one token and walks over its heads
+// with the angles, times the norm's weights, in registers: no barrier anywhere.  A head is
+// held by G = 8, 16 or 32 lanes, eight elements (four pairs) each; the sum of squares is a
+// shuffle tree over those lanes.  Each lane keeps up to 64 bytes of the heads to come in flight
+// through cp.async into slots of shared memory that it alone reads: held in registers,
+// the same bytes left too few warps an SM to cover the memory's latency (158 against
+// 143 us).  32768 tokens of 24 + 24 heads of 128 in fp16, 805 MB: 143 us, 5.6 TB/s, 0.86 of
+// the measured copy rate.
 #include "h3_types.cuh"
 
 namespace h3 {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 constexpr int kRopeThreads = 256;
+// Four CTAs an SM (64 registers a thread) and 64 bytes a lane in flight; three, five or six
+// CTAs and 128 bytes measured up to 10% slower at 32768 tokens of 48 heads.
+constexpr int kRopeCtas = 4;
+constexpr int kRopeSlotBytes = 64;
 
 struct HeadView {
   const void* in;
@@ -30,8 +37,7 @@ struct RopeArgs {
   HeadView q, k;
   int64_t tokens;
   int dim, pairs, axes, pos_kind, norm;
-  int tile_tokens, tile_heads;  // of one CTA
-  uint32_t head_magic;          // ceil(2^32 / tile_heads)
+  int parts;  // lane groups that share the heads of a token
   float eps, inv_dim;
   const void* positions;
   double turns[kMaxPairs];      // frequency / (2 pi)
@@ -40,203 +46,318 @@ struct RopeArgs {
 
 // Angles of far positions need more than 24 bits: the turns are reduced to a fraction of
 // one in 64 bits, and the sine and cosine of that fraction taken in 32.
-H3_DEV float2 pair_angle(const RopeArgs& a, int64_t token, int axis, double turns) {
+H3_DEV void pair_angle(const RopeArgs& a, int64_t token, int axis, double turns, float& c, float& s) {
   const int64_t at = token * a.axes + axis;
   double pos;
   if (a.pos_kind == H3_POS_I32) pos = (double)__ldg(reinterpret_cast<const int32_t*>(a.positions) + at);
   else if (a.pos_kind == H3_POS_I64) pos = (double)__ldg(reinterpret_cast<const long long*>(a.positions) + at);
   else pos = (double)__ldg(reinterpret_cast<const float*>(a.positions) + at);
   const double t = pos * turns;
-  float s, c;
   sincospif(2.0f * (float)(t - rint(t)), &s, &c);
-  return make_float2(c, s);
 }
 
-// The four pairs of a lane: first elements in v[0..3], second in v[4..7] when the pairs
-// are halves apart, (v[2i], v[2i + 1]) otherwise.  VEC: whole 16-byte (or 8-byte) pieces;
-// else one element at a time, any alignment and any head_dim.
+// The eight elements of lane u: four pairs, as v[0..3] = first elements and v[4..7] =
+// second elements, packed two floats to a register pair (half the instructions).  VEC:
+// whole 16-byte (or 8-byte) pieces, a lane's pairs all turned or none; else one element at
+// a time, any alignment and any head_dim.
 template <typename T, bool HALF, bool VEC>
 struct HeadLane {
-  Raw<T, 8> r;        // VEC
-  float x[8];         // !VEC
-
+  // where first (i < 4) or second element i of the lane lies in the head
   H3_DEV static int element(const RopeArgs& a, int u, int i) {
-    if (!HALF) return 8 * u + i;
-    const int p = 4 * u + (i & 3);          // pair p's element i / 4
-    if (p < a.pairs) return i < 4 ? p : p + a.pairs;
-    return 2 * p + (i >> 2);                // behind the turned elements: neighbours
+    const int p = 4 * u + (i & 3);
+    if (HALF && p < a.pairs) return i < 4 ? p : p + a.pairs;
+    return 2 * p + (i >> 2);  // neighbours, also behind the turned halves
   }
-  H3_DEV void load(const RopeArgs& a, const T* p, int u) {
+  // the weight of first or second element i
+  H3_DEV static float weight(const RopeArgs& a, const float* w, int u, int i) {
+    const int e = VEC && HALF && 4 * u >= a.pairs ? 8 * u + i : element(a, u, i);
+    return e < a.dim ? __ldg(w + e) : 0.0f;
+  }
+  // eight values in memory order to pairs and back; behind turned halves the lane is only
+  // scaled, so there the order of its elements does not matter
+  H3_DEV static void to_pairs(const float (&x)[8], f32x2 (&v)[4]) {
+    if (VEC && !HALF) {
+      v[0] = pk2(x[0], x[2]); v[1] = pk2(x[4], x[6]);
+      v[2] = pk2(x[1], x[3]); v[3] = pk2(x[5], x[7]);
+    } else {
+      v[0] = pk2(x[0], x[1]); v[1] = pk2(x[2], x[3]);
+      v[2] = pk2(x[4], x[5]); v[3] = pk2(x[6], x[7]);
+    }
+  }
+  H3_DEV static void load(const RopeArgs& a, const T* p, int u, f32x2 (&v)[4]) {  // !VEC
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = element(a, u, i);
+      x[i] = e < a.dim ? to_f32(p[e]) : 0.0f;
+    }
+    to_pairs(x, v);
+  }
+  H3_DEV static void store(const RopeArgs& a, T* p, int u, const f32x2 (&v)[4]) {
+    float x[8];
+    if (VEC && !HALF) {
+      x[0] = lo2(v[0]); x[2] = hi2(v[0]); x[4] = lo2(v[1]); x[6] = hi2(v[1]);
+      x[1] = lo2(v[2]); x[3] = hi2(v[2]); x[5] = lo2(v[3]); x[7] = hi2(v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = lo2(v[i]);
+        x[2 * i + 1] = hi2(v[i]);
+      }
+    }
     if constexpr (VEC) {
       if (HALF && 4 * u < a.pairs) {
         Raw<T, 4> lo, hi;
-        lo.load(p + 4 * u);
-        hi.load(p + a.pairs + 4 * u);
-#pragma unroll
-        for (int i = 0; i < Raw<T, 4>::kWords; ++i) {
-          r.w[i] = lo.w[i];
-          r.w[Raw<T, 4>::kWords + i] = hi.w[i];
-        }
-      } else {
-        r.load(p + 8 * u);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = element(a, u, i);
-        x[i] = e < a.dim ? to_f32(p[e]) : 0.0f;
-      }
-    }
-  }
-  H3_DEV void values(float* v) const {
-    if constexpr (VEC) {
-      r.unpack(v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = x[i];
-    }
-  }
-  H3_DEV static void store(const RopeArgs& a, T* p, int u, const float* v) {
-    if constexpr (VEC) {
-      if (HALF && 4 * u < a.pairs) {
-        Raw<T, 4> lo, hi;
-        lo.pack(v);
-        hi.pack(v + 4);
+        lo.pack(x);
+        hi.pack(x + 4);
         lo.store(p + 4 * u);
         hi.store(p + a.pairs + 4 * u);
       } else {
         Raw<T, 8> o;
-        o.pack(v);
+        o.pack(x);
         o.store(p + 8 * u);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int e = element(a, u, i);
-        if (e < a.dim) p[e] = from_f32<T>(v[i]);
+        if (e < a.dim) p[e] = from_f32<T>(x[i]);
       }
     }
-  }
-  // weight of element i of this lane; VEC keeps neighbours behind the turned elements in
-  // memory order, so there the index is the memory's
-  H3_DEV static int weight_index(const RopeArgs& a, int u, int i) {
-    if (VEC && HALF && 4 * u >= a.pairs) return 8 * u + i;
-    return element(a, u, i);
   }
 };
 
-template <typename T, bool HALF, bool VEC, int G>
-__global__ void __launch_bounds__(kRopeThreads, VEC ? 4 : 2)
-    rope_kernel(const __grid_constant__ RopeArgs a) {
-  // A lane reads its four angles and its eight weights as 16-byte words, the lanes of a
-  // group side by side: [buffer][token][pair & 2][lane] and [q, k][half][lane].
-  __shared__ __align__(16) float4 turn[2][kRopeThreads / 2 + 64];
-  __shared__ __align__(16) float4 weight[2][2][32];
-  constexpr int kGroups = kRopeThreads / G;
-  constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;  // heads a lane group has in flight, 64 bytes a lane
-  using Lane = HeadLane<T, HALF, VEC>;
-  const int u = threadIdx.x % G, group = threadIdx.x / G;
-  const int quads = (a.pairs + 3) / 4;  // lanes with turned pairs
-  const int head0 = blockIdx.y * a.tile_heads;
-  const int heads = min(a.tile_heads, a.q.heads + a.k.heads - head0);
-  const bool live = 8 * u < a.dim;
+// (v1, v2) -> inv * (x1 cw1 - x2 sw2, x2 cw2 + x1 sw1): the angles of a lane's pairs with
+// the norm's weights taken in (sw2 carries the minus).
+struct Turn {
+  f32x2 cw1[2], sw1[2], cw2[2], sw2[2];
+};
 
-  const bool weighted = a.norm && (a.q.weight != nullptr || a.k.weight != nullptr);
-  if (weighted) {
-    for (int i = threadIdx.x; i < 512; i += kRopeThreads) {
-      const float* w = i < 256 ? a.q.weight : a.k.weight;
-      const int lane = (i & 255) >> 3, e = Lane::weight_index(a, lane, i & 7);
-      reinterpret_cast<float*>(&weight[i >> 8][(i >> 2) & 1][lane])[i & 3] =
-          w != nullptr && e < a.dim ? __ldg(w + e) : 1.0f;
+template <typename T, bool HALF, bool VEC>
+H3_DEV void weigh(const RopeArgs& a, const float* weight, int u, const float (&c)[4],
+                  const float (&s)[4], Turn& t) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (a.norm && weight != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        w[e] = HeadLane<T, HALF, VEC>::weight(a, weight, u, 2 * i + e);
+        w[2 + e] = HeadLane<T, HALF, VEC>::weight(a, weight, u, 4 + 2 * i + e);
+      }
+    }
+    t.cw1[i] = pk2(c[2 * i] * w[0], c[2 * i + 1] * w[1]);
+    t.sw1[i] = pk2(s[2 * i] * w[0], s[2 * i + 1] * w[1]);
+    t.cw2[i] = pk2(c[2 * i] * w[2], c[2 * i + 1] * w[3]);
+    t.sw2[i] = pk2(-s[2 * i] * w[2], -s[2 * i + 1] * w[3]);
+  }
+}
+
+// Norm and turn of one head; every lane of the warp calls it.
+template <bool VEC, int G>
+H3_DEV void turn_head(const RopeArgs& a, int u, const Turn& t, f32x2 (&x)[4]) {
+  if (a.norm) {
+    f32x2 sq = mul2(x[0], x[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) sq = fma2(x[i], x[i], sq);
+    float sum = lo2(sq) + hi2(sq);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const f32x2 inv = dup2(rsqrtf(__fmaf_rn(sum, a.inv_dim, a.eps)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], inv);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 x1 = x[i], x2 = x[i + 2];
+    x[i] = mul2(x1, t.cw1[i]);
+    x[i + 2] = mul2(x2, t.cw2[i]);
+    // an element that is not turned must not meet an infinite neighbour times 0
+    if (VEC ? 4 * u < a.pairs : 4 * u + 2 * i + 1 < a.pairs) {
+      x[i] = fma2(x2, t.sw2[i], x[i]);
+      x[i + 2] = fma2(x1, t.sw1[i], x[i + 2]);
+    } else if (!VEC && 4 * u + 2 * i < a.pairs) {  // the first of the two alone
+      x[i] = pk2(__fmaf_rn(lo2(x2), lo2(t.sw2[i]), lo2(x[i])), hi2(x[i]));
+      x[i + 2] = pk2(__fmaf_rn(lo2(x1), lo2(t.sw1[i]), lo2(x[i + 2])), hi2(x[i + 2]));
     }
   }
-  // this thread's pair of the tile's angles
-  const int my_tok = threadIdx.x / a.pairs, my_pair = threadIdx.x - my_tok * a.pairs;
-  const double my_turns = my_tok < a.tile_tokens ? a.turns[my_pair] : 0.0;
-  const int my_axis = my_tok < a.tile_tokens ? a.axis[my_pair] : 0;
-  float2* my_slot = reinterpret_cast<float2*>(
-      &turn[0][(my_tok * 2 + ((my_pair >> 1) & 1)) * quads + (my_pair >> 2)]) + (my_pair & 1);
+}
 
-  int buffer = 0;
-  for (int64_t tile = blockIdx.x; tile * a.tile_tokens < a.tokens; tile += gridDim.x, buffer ^= 1) {
-    const int64_t token0 = tile * a.tile_tokens;
-    const int tokens = (int)min((int64_t)a.tile_tokens, a.tokens - token0);
-    const int items = tokens * a.tile_heads;
-    if (my_tok < tokens)
-      my_slot[buffer * (sizeof(turn[0]) / sizeof(float2))] =
-          pair_angle(a, token0 + my_tok, my_axis, my_turns);
-    // one barrier a tile: the buffer written next was last read before this one
-    __syncthreads();
-    const T* q_in = reinterpret_cast<const T*>(a.q.in) + token0 * a.q.in_token;
-    const T* k_in = reinterpret_cast<const T*>(a.k.in) + token0 * a.k.in_token;
-    T* q_out = reinterpret_cast<T*>(a.q.out) + token0 * a.q.out_token;
-    T* k_out = reinterpret_cast<T*>(a.k.out) + token0 * a.k.out_token;
+// A round of a CTA: one item for each of its lane groups, an item being a token and the
+// part of its heads (part, part + parts, ... of q, then of k) that the group takes.
+struct Round {
+  bool here;
+  int64_t token;
+  int part;
 
-    // every lane of the CTA makes every step (the shuffles need them all); `head` is -1
-    // where there is nothing to do
-    for (int base = group; base - group < items; base += kGroups * kAhead) {
-      Lane lane[kAhead];
-      int tok[kAhead], head[kAhead];
+  H3_DEV Round(const RopeArgs& a, int item, bool live) {
+    const int items = (int)a.tokens * a.parts;
+    here = item < items && live;
+    token = item < items ? item / a.parts : 0;
+    part = item < items ? item - (int)token * a.parts : 0;
+  }
+  H3_DEV int count(const RopeArgs& a, const HeadView& v) const {
+    return here ? (v.heads - part + a.parts - 1) / a.parts : 0;
+  }
+};
+
+H3_DEV void lane_angles(const RopeArgs& a, int64_t token, int u, const double* turns,
+                        const unsigned char* axis, float (&c)[4], float (&s)[4]) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const int it = base + j * kGroups;
-        // it / tile_heads: exact, their product is below 2^32; 2^32 itself has no 32-bit form
-        tok[j] = a.head_magic != 0 ? (int)__umulhi((uint32_t)it, a.head_magic) : it;
-        head[j] = it - tok[j] * a.tile_heads;
-        head[j] = it < items && head[j] < heads && live ? head[j] + head0 : -1;
-        if (head[j] >= 0) {
-          const bool is_k = head[j] >= a.q.heads;
-          const T* in = is_k ? k_in : q_in;
-          in += (int64_t)tok[j] * (is_k ? a.k.in_token : a.q.in_token) +
-                (int64_t)(is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.in_head : a.q.in_head);
-          lane[j].load(a, in, u);
+  for (int i = 0; i < 4; ++i) {
+    c[i] = 1.0f;
+    s[i] = 0.0f;
+    if (4 * u + i < a.pairs) pair_angle(a, token, axis[4 * u + i], turns[4 * u + i], c[i], s[i]);
+  }
+}
+
+H3_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+H3_DEV void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// Vector form.  Loops over rounds, tensors and steps are the same for every lane of the
+// CTA, so that every lane makes every step (the shuffles need them all).
+template <typename T, bool HALF, int G>
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
+    rope_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kGroups = kRopeThreads / G;
+  constexpr int kWords = sizeof(T) / 2;             // 16-byte words of a lane's eight values
+  constexpr int kSlots = kRopeSlotBytes / (16 * kWords);
+  using Lane = HeadLane<T, HALF, true>;
+  __shared__ __align__(16) uint4 ring[kSlots][kWords][kRopeThreads];
+  // the plan, where lanes can read different entries of it at once
+  __shared__ double turns[kMaxPairs];
+  __shared__ unsigned char axis[kMaxPairs];
+  for (int i = threadIdx.x; i < kMaxPairs; i += kRopeThreads) {
+    turns[i] = a.turns[i];
+    axis[i] = a.axis[i];
+  }
+  __syncthreads();
+  const int u = threadIdx.x % G, group = threadIdx.x / G;
+  const bool live = 8 * u < a.dim, turned = 4 * u < a.pairs;
+  const int rounds = ((int)a.tokens * a.parts + kGroups - 1) / kGroups;
+  const int tensors = a.k.heads > 0 ? 2 : 1;
+
+  // the fetching side, kSlots - 1 steps ahead
+  int f_round = blockIdx.x, f_which = 0, f_left = 0, f_count = 0;
+  const T* f_in = nullptr;
+  int64_t f_step = 0;
+  const auto f_open = [&]() {
+    const HeadView& v = f_which ? a.k : a.q;
+    const Round r(a, f_round * kGroups + group, live);
+    f_left = (v.heads + a.parts - 1) / a.parts;
+    f_count = r.count(a, v);
+    f_step = (int64_t)a.parts * v.in_head;
+    f_in = reinterpret_cast<const T*>(v.in) + r.token * v.in_token + (int64_t)r.part * v.in_head;
+  };
+  const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(&ring[0][0][threadIdx.x]);
+  const auto fetch = [&](int slot) {
+    if (f_round < rounds) {
+      if (f_count > 0) {
+        const uint32_t dst = my_ring + slot * (uint32_t)sizeof(ring[0]);
+        if (HALF && turned) {
+          if (sizeof(T) == 2) {
+            cp_async8(dst, f_in + 4 * u);
+            cp_async8(dst + 8, f_in + a.pairs + 4 * u);
+          } else {
+            cp_async16(dst, f_in + 4 * u);
+            cp_async16(dst + (uint32_t)sizeof(ring[0][0]), f_in + a.pairs + 4 * u);
+          }
+        } else {
+          cp_async16(dst, f_in + 8 * u);
+          if (sizeof(T) == 4) cp_async16(dst + (uint32_t)sizeof(ring[0][0]), f_in + 8 * u + 4);
         }
       }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        float v[8];
-        const bool is_k = head[j] >= a.q.heads;
-        if (head[j] >= 0) {
-          lane[j].values(v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      f_in += f_step;
+      --f_count;
+      if (--f_left == 0) {
+        if (++f_which == tensors) {
+          f_which = 0;
+          f_round += gridDim.x;
         }
-        if (a.norm) {
-          float sum = 0.0f;
+        if (f_round < rounds) f_open();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  f_open();
+#pragma unroll 1
+  for (int i = 0; i < kSlots - 1; ++i) fetch(i);
+
+  int slot = 0;
+#pragma unroll 1
+  for (int round = blockIdx.x; round < rounds; round += gridDim.x) {
+    const Round r(a, round * kGroups + group, live);
+    float c[4], s[4];
+    lane_angles(a, r.token, u, turns, axis, c, s);
+#pragma unroll 1
+    for (int which = 0; which < tensors; ++which) {
+      const HeadView& v = which ? a.k : a.q;
+      const int count = r.count(a, v);
+      const int steps = (v.heads + a.parts - 1) / a.parts;
+      Turn t;
+      weigh<T, HALF, true>(a, v.weight, u, c, s, t);
+      const int64_t out_step = (int64_t)a.parts * v.out_head;
+      T* out = reinterpret_cast<T*>(v.out) + r.token * v.out_token + (int64_t)r.part * v.out_head;
+#pragma unroll 1
+      for (int h = 0; h < steps; ++h) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        f32x2 x[4] = {0, 0, 0, 0};
+        if (h < count) {
+          Raw<T, 8> raw;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum = __fmaf_rn(v[i], v[i], sum);
-#pragma unroll
-          for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          const float inv = rsqrtf(__fmaf_rn(sum, a.inv_dim, a.eps));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= inv;
-          if (weighted) {
-            const float4 w0 = weight[is_k][0][u], w1 = weight[is_k][1][u];
-            v[0] *= w0.x; v[1] *= w0.y; v[2] *= w0.z; v[3] *= w0.w;
-            v[4] *= w1.x; v[5] *= w1.y; v[6] *= w1.z; v[7] *= w1.w;
+          for (int w = 0; w < kWords; ++w) {
+            const uint4 q = ring[slot][w][threadIdx.x];
+            raw.w[4 * w] = q.x; raw.w[4 * w + 1] = q.y; raw.w[4 * w + 2] = q.z; raw.w[4 * w + 3] = q.w;
           }
+          float f[8];
+          raw.unpack(f);
+          Lane::to_pairs(f, x);
         }
-        if (head[j] < 0) continue;
-        if (u < quads) {
-          const float4* t = &turn[buffer][tok[j] * 2 * quads + u];
-          const float4 t0 = t[0], t1 = t[quads];
-          const float c[4] = {t0.x, t0.z, t1.x, t1.z}, s[4] = {t0.y, t0.w, t1.y, t1.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!VEC && 4 * u + i >= a.pairs) continue;
-            if (VEC && !HALF && 4 * u + i >= a.pairs) continue;
-            float& v1 = v[HALF ? i : 2 * i];
-            float& v2 = v[HALF ? i + 4 : 2 * i + 1];
-            const float r1 = __fmaf_rn(v1, c[i], -(v2 * s[i]));
-            v2 = __fmaf_rn(v2, c[i], v1 * s[i]);
-            v1 = r1;
-          }
-        }
-        T* out = is_k ? k_out : q_out;
-        out += (int64_t)tok[j] * (is_k ? a.k.out_token : a.q.out_token) +
-               (int64_t)(is_k ? head[j] - a.q.heads : head[j]) * (is_k ? a.k.out_head : a.q.out_head);
-        Lane::store(a, out, u, v);
+        // the slot of the step before: its values were used up there
+        fetch((slot + kSlots - 1) % kSlots);
+        slot = (slot + 1) % kSlots;
+        turn_head<true, G>(a, u, t, x);
+        if (h < count) Lane::store(a, out, u, x);
+        out += out_step;
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Any alignment, any head_dim: one element at a time.
+template <typename T, bool HALF, int G>
+__global__ void __launch_bounds__(kRopeThreads, 2)
+    rope_scalar_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kGroups = kRopeThreads / G;
+  using Lane = HeadLane<T, HALF, false>;
+  const int u = threadIdx.x % G, group = threadIdx.x / G;
+  const bool live = 8 * u < a.dim;
+  const int rounds = ((int)a.tokens * a.parts + kGroups - 1) / kGroups;
+#pragma unroll 1
+  for (int round = blockIdx.x; round < rounds; round += gridDim.x) {
+    const Round r(a, round * kGroups + group, live);
+    float c[4], s[4];
+    lane_angles(a, r.token, u, a.turns, a.axis, c, s);
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const HeadView& v = which ? a.k : a.q;
+      const int count = r.count(a, v);
+      const int steps = (v.heads + a.parts - 1) / a.parts;
+      Turn t;
+      weigh<T, HALF, false>(a, v.weight, u, c, s, t);
+      for (int h = 0; h < steps; ++h) {
+        const int64_t head = r.part + (int64_t)h * a.parts;
+        f32x2 x[4] = {0, 0, 0, 0};
+        if (h < count)
+          Lane::load(a, reinterpret_cast<const T*>(v.in) + r.token * v.in_token + head * v.in_head, u, x);
+        turn_head<false, G>(a, u, t, x);
+        if (h < count)
+          Lane::store(a, reinterpret_cast<T*>(v.out) + r.token * v.out_token + head * v.out_head, u, x);
       }
     }
   }
@@ -244,22 +365,17 @@ __global__ void __launch_bounds__(kRopeThreads, VEC ? 4 : 2)
 
 template <typename T, bool HALF, bool VEC, int G>
 int launch_rope(RopeArgs& a, int sms, cudaStream_t stream) {
-  // A tile is as many tokens as give every thread one angle; with too few tiles for the
-  // SMs it shrinks, at last to a part of one token's heads (rounds of the lane groups).
+  // One lane group a token; with fewer tokens than lane groups on the GPU the heads are
+  // split too, down to four a group, as the sines of a token cost about three heads.
   constexpr int kGroups = kRopeThreads / G;
-  const int heads = a.q.heads + a.k.heads;
-  int tokens = std::max<int>(1, kRopeThreads / a.pairs);
-  tokens = std::min<int>(tokens, 16);
-  while (tokens > 1 && (a.tokens + tokens - 1) / tokens < 2 * sms) tokens /= 2;
-  a.tile_tokens = tokens;
-  a.tile_heads = heads;
-  const int64_t tiles = (a.tokens + tokens - 1) / tokens;
-  if (tokens == 1 && tiles < sms)
-    a.tile_heads = std::min<int>(heads, kGroups * std::max<int>(1, (int)(tiles * heads / ((int64_t)sms * kGroups))));
-  const int splits = (heads + a.tile_heads - 1) / a.tile_heads;
-  a.head_magic = (uint32_t)(((1ull << 32) + a.tile_heads - 1) / a.tile_heads);
-  const int grid = (int)std::min<int64_t>(tiles, (int64_t)sms * (VEC ? 4 : 2));
-  rope_kernel<T, HALF, VEC, G><<<dim3(grid, splits), kRopeThreads, 0, stream>>>(a);
+  const int heads = std::max(a.q.heads, a.k.heads);
+  const int ctas = VEC ? kRopeCtas : 2;
+  const int64_t room = (int64_t)sms * ctas * kGroups;
+  a.parts = (int)std::min<int64_t>((heads + 3) / 4, std::max<int64_t>(1, room / a.tokens));
+  const int64_t rounds = (a.tokens * a.parts + kGroups - 1) / kGroups;
+  const int grid = (int)std::min<int64_t>(rounds, (int64_t)sms * ctas);
+  if constexpr (VEC) rope_kernel<T, HALF, G><<<grid, kRopeThreads, 0, stream>>>(a);
+  else rope_scalar_kernel<T, HALF, G><<<grid, kRopeThreads, 0, stream>>>(a);
   return h3host::check_launch();
 }
 
@@ -272,9 +388,9 @@ int launch_rope_width(RopeArgs& a, int sms, cudaStream_t stream) {
 
 template <typename T>
 int launch_rope_type(RopeArgs& a, bool half, int sms, cudaStream_t stream) {
-  // whole 16-byte pieces: every head starts on a 16-byte boundary, is a multiple of eight
-  // elements, and halves (if paired so) are multiples of four pairs
-  bool vec = a.dim % 8 == 0 && (!half || a.pairs % 4 == 0);
+  // whole 16-byte pieces: every head starts on a 16-byte boundary and has a multiple of
+  // eight elements and of four turned pairs
+  bool vec = a.dim % 8 == 0 && a.pairs % 4 == 0;
   for (const HeadView* v : {&a.q, &a.k}) {
     if (v->heads == 0) continue;
     vec = vec && h3host::aligned(v->in, 16) && h3host::aligned(v->out, 16);
@@ -301,7 +417,7 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
   if (k == nullptr) k_heads = 0;
   if (q == nullptr || q_out == nullptr || (k != nullptr && k_out == nullptr) || tokens < 0 ||
       q_heads < 1 || q_heads > 4096 || k_heads < 0 || k_heads > 4096 || head_dim < 2 ||
-      head_dim > 2 * kMaxPairs || positions == nullptr || axes < 1 || axes > 255 ||
+      head_dim > 2 * kMaxPairs || tokens > (1 << 30) || positions == nullptr || axes < 1 || axes > 255 ||
       turns == nullptr || axis == nullptr || pairs < 1 || 2 * pairs > head_dim ||
       pos_kind < H3_POS_I32 || pos_kind > H3_POS_F32 || type < H3_TYPE_F32 || type > H3_TYPE_BF16)
     return H3_ERR_INVALID;
