@@ -5,6 +5,13 @@
 // with x' rounded once to the residual's type, and h either rounded once to that type or
 // (rotated by ConvRot256 and) quantised per row to INT8.  Statistics, x' and h are held
 // in fp32 between the two roundings.
+//
+// Bound by HBM: x and the branch are read once, x' and h (or the codes) written once; the
+// row lives in registers from its load to its last store, eight values a thread, one CTA a
+// row.  What else a row needs is kept off the memory's path: the modulation tables and the
+// norms' weights, four times the row's own bytes, are folded into three factors a value
+// and stay in registers until a row has another label, and rows to come are fetched by
+// cp.async into slots of shared memory that only the fetching thread reads.
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -32,123 +39,448 @@ struct ResidualNorm {
   int* err;
 };
 
-H3_DEV float norm_block_sum(float v, float* red) {
+// Sum or maximum over the CTA.  `red` has two rows of 32, used in turn: one barrier a call,
+// as a row is written again only after the barrier of the call between.
+struct BlockReduce {
+  float* red;
+  int turn;
+
+  H3_DEV float* publish(float v) {
+    float* r = red + 32 * turn;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return r;
+  }
+  H3_DEV float sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.0f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += red[w];
-  return t;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (blockDim.x == 32) return v;
+    const float* r = publish(v);
+    float t = 0.0f;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += r[w];
+    return t;
+  }
+  // NAN_WINS: NaN if any value is; else values that are NaN are left out
+  template <bool NAN_WINS>
+  H3_DEV float max(float v) {
+    const auto larger = [](float a, float b) { return NAN_WINS ? max_abs2_nan(0.0f, a, b) : fmaxf(a, b); };
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (blockDim.x == 32) return v;
+    const float* r = publish(v);
+    float t = 0.0f;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t = larger(t, r[w]);
+    return t;
+  }
+};
+
+H3_DEV f32x2 shfl2(f32x2 v, int mask) {
+  return pk2(__shfl_xor_sync(0xffffffffu, lo2(v), mask), __shfl_xor_sync(0xffffffffu, hi2(v), mask));
 }
 
-H3_DEV float norm_block_max(float v, float* red) {
-  v = warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.0f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t = fmaxf(t, red[w]);
-  return t;
+// The regular 256-point rotation of the 256 values of a warp, v[i] = (value i, value i + 4)
+// of lane's eight.  One radix-4 stage takes (x0, x1, x2, x3) to
+//   (x0 + x1) + (x2 - x3), (x0 + x1) - (x2 - x3), (x0 - x1) + (x2 + x3), (x2 + x3) - (x0 - x1)
+// i.e. y_i = x_i + x_(i^1) + x_(i^2) - x_(i^3).  The first digit of a value's index lies in
+// the registers, the second has one bit in the pair and one in the lane, the others are lane
+// bits, so they go by shuffles (4.5 a value in all; through shared memory the rotation
+// needs four accesses a value and a barrier for each of its two transposes).
+H3_DEV void convrot256_warp(f32x2 (&v)[4]) {
+  {
+    const f32x2 s01 = add2(v[0], v[1]), d01 = sub2(v[0], v[1]);
+    const f32x2 s23 = add2(v[2], v[3]), d23 = sub2(v[2], v[3]);
+    v[0] = add2(s01, d23); v[1] = sub2(s01, d23);
+    v[2] = add2(d01, s23); v[3] = sub2(s23, d01);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float s = lo2(v[i]) + hi2(v[i]);
+    const float d = __shfl_xor_sync(0xffffffffu, lo2(v[i]) - hi2(v[i]), 1);
+    v[i] = pk2(s + d, s - d);
+  }
+#pragma unroll
+  for (int bit = 2; bit <= 8; bit *= 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x2 p = shfl2(v[i], bit);
+      v[i] = add2(add2(v[i], p), shfl2(sub2(v[i], p), 2 * bit));
+    }
+  }
+  const f32x2 sixteenth = dup2(0.0625f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], sixteenth);
 }
 
-// Normalises row[0, width) in place (each thread its own elements).
-H3_DEV void norm_row(float* row, int64_t width, float inv_width, int kind, const float* w,
-                     const float* b, float eps, float* red) {
-  if (kind == H3_NORM_NONE) return;
-  float mean = 0.0f;
+// Where value j of a thread's chunk lies in the row.  Eight neighbours where the row allows
+// it (VEC: in 16-byte words); rows of a width that is no multiple of eight are dealt value
+// by value over the threads, so that a warp's accesses are neighbours.
+struct Deal {
+  int width, thread_step, value_step, chunk_step;
+  H3_DEV int at(int chunk, int j) const {
+    return threadIdx.x * thread_step + j * value_step + chunk * chunk_step;
+  }
+};
+
+// The pairs (value j, value j + 4) of a chunk; values outside the row read as `fill`.
+template <bool VEC>
+H3_DEV void load_table(const float* t, const Deal& d, int chunk, bool in_row, float fill, f32x2 (&v)[4]) {
+  float x[8];
+  if constexpr (VEC) {
+    if (in_row) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(t + d.at(chunk, 0)));
+      const float4 b = __ldg(reinterpret_cast<const float4*>(t + d.at(chunk, 0)) + 1);
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fill;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = d.at(chunk, j) < d.width ? __ldg(t + d.at(chunk, j)) : fill;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pk2(x[i], x[i + 4]);
+}
+
+template <typename T, bool VEC>
+H3_DEV void load_chunk(const T* row, const Deal& d, int chunk, bool in_row, f32x2 (&v)[4]) {
+  float x[8];
+  if constexpr (VEC) {
+    if (in_row) {
+      Raw<T, 8> r;
+      r.load(row + d.at(chunk, 0));
+      r.unpack(x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = d.at(chunk, j) < d.width ? to_f32(row[d.at(chunk, j)]) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pk2(x[i], x[i + 4]);
+}
+
+template <typename T, bool VEC>
+H3_DEV void store_chunk(T* row, const Deal& d, int chunk, bool in_row, const f32x2 (&v)[4]) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = lo2(v[i]);
+    x[i + 4] = hi2(v[i]);
+  }
+  if constexpr (VEC) {
+    if (in_row) {
+      Raw<T, 8> r;
+      r.pack(x);
+      r.store(row + d.at(chunk, 0));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (d.at(chunk, j) < d.width) row[d.at(chunk, j)] = from_f32<T>(x[j]);
+  }
+}
+
+// What a thread's values of a chunk are multiplied by and shifted by, for one label.
+struct Factors {
+  f32x2 gate[4];   // gate * post weight
+  f32x2 scale[4];  // pre weight * (1 + scale)
+  f32x2 shift[4];  // pre bias * (1 + scale) + shift
+};
+
+template <bool VEC>
+H3_DEV void load_factors(const ResidualNorm& a, const Deal& d, int chunk, bool in_row, int64_t lab, Factors& f) {
+  f32x2 t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.gate[i] = f.scale[i] = dup2(1.0f);
+    f.shift[i] = 0;
+  }
+  if (a.gate != nullptr) load_table<VEC>(a.gate + lab * a.gate_ld, d, chunk, in_row, 0.0f, f.gate);
+  if (a.post_weight != nullptr) {
+    load_table<VEC>(a.post_weight, d, chunk, in_row, 0.0f, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.gate[i] = mul2(f.gate[i], t[i]);
+  }
+  if (a.pre_kind == H3_NORM_NONE) return;
+  if (a.scale != nullptr) {
+    load_table<VEC>(a.scale + lab * a.scale_ld, d, chunk, in_row, 0.0f, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.scale[i] = add2(f.scale[i], t[i]);
+  }
+  if (a.shift != nullptr) load_table<VEC>(a.shift + lab * a.shift_ld, d, chunk, in_row, 0.0f, f.shift);
+  if (a.pre_bias != nullptr) {
+    load_table<VEC>(a.pre_bias, d, chunk, in_row, 0.0f, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.shift[i] = fma2(t[i], f.scale[i], f.shift[i]);
+  }
+  if (a.pre_weight != nullptr) {
+    load_table<VEC>(a.pre_weight, d, chunk, in_row, 0.0f, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.scale[i] = mul2(f.scale[i], t[i]);
+  }
+}
+
+// (v - mean) * inv of a row, in place; values outside the row are 0 before and after.  The
+// variance of LayerNorm is taken around the mean, in a second sum.
+template <int NC, bool VEC>
+H3_DEV void normalise(f32x2 (&v)[NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
+                      int kind, float eps, BlockReduce& reduce) {
   if (kind == H3_NORM_LAYER) {
-    float s = 0.0f;
-    for (int64_t c = threadIdx.x; c < width; c += blockDim.x) s += row[c];
-    mean = norm_block_sum(s, red) * inv_width;
+    f32x2 t = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t = add2(t, v[c][i]);
+    const f32x2 mean = dup2(reduce.sum(lo2(t) + hi2(t)) * a.inv_width);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 m = sub2(v[c][i], mean);
+        if (VEC) {
+          v[c][i] = in_row[c] ? m : 0;
+        } else {
+          v[c][i] = pk2(d.at(c, i) < d.width ? lo2(m) : 0.0f, d.at(c, i + 4) < d.width ? hi2(m) : 0.0f);
+        }
+      }
   }
-  float s = 0.0f;
-  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) {
-    const float d = row[c] - mean;
-    s = __fmaf_rn(d, d, s);
-  }
-  const float inv = __frsqrt_rn(__fmaf_rn(norm_block_sum(s, red), inv_width, eps));
-  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) {
-    float v = (row[c] - mean) * inv;
-    if (w != nullptr) v *= __ldg(w + c);
-    if (b != nullptr) v += __ldg(b + c);
-    row[c] = v;
-  }
+  f32x2 t = 0;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t = fma2(v[c][i], v[c][i], t);
+  const f32x2 inv = dup2(rsqrtf(__fmaf_rn(reduce.sum(lo2(t) + hi2(t)), a.inv_width, eps)));
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], inv);
 }
 
-template <typename XT, typename BT>
-__global__ void __launch_bounds__(256) residual_norm_kernel(const ResidualNorm a) {
-  extern __shared__ __align__(16) float row[];
-  __shared__ float red[8];
-  const XT* x = reinterpret_cast<const XT*>(a.x);
-  const BT* branch = reinterpret_cast<const BT*>(a.branch);
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    int64_t lab = a.labels != nullptr ? (int64_t)__ldg(a.labels + r) : 0;
+// The code of a value of a row that holds infinities or NaN (rare: kept out of line, where
+// it costs the other rows no registers).
+__device__ __noinline__ uint32_t any_code(float v, float scale) {
+  return (uint32_t)(int)quantize_code(v, scale, 0);
+}
+
+// NC chunks of eight values a thread.  NC 1: the factors stay in registers, and (VEC) rows
+// are fetched SLOTS - 1 ahead.
+template <typename XT, typename BT, int NC, bool VEC, bool QUANT, int SLOTS>
+__global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ ResidualNorm a,
+                                                             const Deal d) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  __shared__ float red[64];
+  constexpr bool kRing = VEC && NC == 1;
+  constexpr int kWordsX = sizeof(XT) / 2, kWordsB = sizeof(BT) / 2;  // 16-byte words of a chunk
+  BlockReduce reduce{red, 0};
+  bool in_row[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) in_row[c] = d.at(c, 0) < d.width;
+  const bool branched = a.branch != nullptr;
+
+  // a slot: the words of x, then of the branch, each a word a thread side by side
+  const uint32_t word = blockDim.x * 16, slot_bytes = word * (kWordsX + kWordsB);
+  const uint32_t mine = kRing ? (uint32_t)__cvta_generic_to_shared(slots) + threadIdx.x * 16 : 0;
+  const auto fetch = [&](int64_t row, int slot) {
+    if (row < a.rows && in_row[0]) {
+      const uint32_t dst = mine + slot * slot_bytes;
+      const XT* x = reinterpret_cast<const XT*>(a.x) + row * a.width + d.at(0, 0);
+#pragma unroll
+      for (int w = 0; w < kWordsX; ++w) cp_async16(dst + w * word, x + w * (16 / sizeof(XT)));
+      if (branched) {
+        const BT* b = reinterpret_cast<const BT*>(a.branch) + row * a.width + d.at(0, 0);
+#pragma unroll
+        for (int w = 0; w < kWordsB; ++w)
+          cp_async16(dst + (kWordsX + w) * word, b + w * (16 / sizeof(BT)));
+      }
+    }
+    cp_async_commit();
+  };
+  if (kRing) {
+#pragma unroll
+    for (int i = 0; i < SLOTS - 1; ++i) fetch(blockIdx.x + (int64_t)i * gridDim.x, i);
+  }
+
+  Factors f;
+  int64_t held = -1;
+  int slot = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    int64_t lab = a.labels != nullptr ? (int64_t)__ldg(a.labels + row) : 0;
     if (lab < 0 || lab >= a.mod_rows) {
       report_error(a.err, H3_ERR_INVALID);
       lab = 0;
     }
-    const int64_t base = r * a.width;
-    if (branch != nullptr) {
-      for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x) row[c] = to_f32(branch[base + c]);
-      norm_row(row, a.width, a.inv_width, a.post_kind, a.post_weight, a.post_bias, a.post_eps, red);
+    if (NC == 1 && lab != held) {
+      load_factors<VEC>(a, d, 0, in_row[0], lab, f);
+      held = lab;
     }
-    for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x) {
-      float v = to_f32(x[base + c]);
-      if (branch != nullptr) {
-        const float g = a.gate != nullptr ? __ldg(a.gate + lab * a.gate_ld + c) : 1.0f;
-        v = __fmaf_rn(g, row[c], a.residual_scale * v);
-        reinterpret_cast<XT*>(a.out)[base + c] = from_f32<XT>(v);
+    const int64_t base = row * a.width;
+    const uint8_t* p = slots + slot * slot_bytes + threadIdx.x * 16;
+    const auto from_slot = [&](auto type, int first, f32x2 (&v)[4]) {
+      using T = decltype(type);
+      Raw<T, 8> r;
+      float t[8];
+#pragma unroll
+      for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+        *reinterpret_cast<uint4*>(&r.w[4 * w]) = *reinterpret_cast<const uint4*>(p + (first + w) * word);
+      r.unpack(t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = in_row[0] ? pk2(t[i], t[i + 4]) : 0;
+    };
+    if constexpr (kRing) cp_async_wait<SLOTS - 2>();
+    f32x2 v[NC][4];  // the branch, then x', then h
+    if (branched) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (kRing) from_slot(BT(), kWordsX, v[0]);
+        else load_chunk<BT, VEC>(reinterpret_cast<const BT*>(a.branch) + base, d, c, in_row[c], v[c]);
       }
-      row[c] = v;
+      if (a.post_kind != H3_NORM_NONE)
+        normalise<NC, VEC>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
+      const f32x2 rs = dup2(a.residual_scale);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        f32x2 x[4];
+        if constexpr (kRing) from_slot(XT(), 0, x);
+        else load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], x);
+        if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c][i] = fma2(f.gate[i], v[c][i], mul2(x[i], rs));
+        if (a.post_bias != nullptr) {  // + gate * bias
+          f32x2 b[4], g[4] = {dup2(1.0f), dup2(1.0f), dup2(1.0f), dup2(1.0f)};
+          load_table<VEC>(a.post_bias, d, c, in_row[c], 0.0f, b);
+          if (a.gate != nullptr) load_table<VEC>(a.gate + lab * a.gate_ld, d, c, in_row[c], 0.0f, g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[c][i] = fma2(g[i], b[i], v[c][i]);
+        }
+        store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.out) + base, d, c, in_row[c], v[c]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if constexpr (kRing) from_slot(XT(), 0, v[0]);
+        else load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], v[c]);
+      }
+    }
+    if constexpr (kRing) {
+      // the slot of the row before, whose values were used up there
+      fetch(row + (int64_t)(SLOTS - 1) * gridDim.x, slot == 0 ? SLOTS - 1 : slot - 1);
+      slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
     if (a.pre_kind == H3_NORM_NONE) continue;
-    norm_row(row, a.width, a.inv_width, a.pre_kind, a.pre_weight, a.pre_bias, a.pre_eps, red);
-    for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x) {
-      float v = row[c];
-      const float f = a.scale != nullptr ? 1.0f + __ldg(a.scale + lab * a.scale_ld + c) : 1.0f;
-      v = __fmaf_rn(v, f, a.shift != nullptr ? __ldg(a.shift + lab * a.shift_ld + c) : 0.0f);
-      row[c] = v;
-      if (a.h != nullptr) reinterpret_cast<XT*>(a.h)[base + c] = from_f32<XT>(v);
+    normalise<NC, VEC>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], f.scale[i], f.shift[i]);
+      if (!QUANT) store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.h) + base, d, c, in_row[c], v[c]);
     }
-    if (a.q == nullptr) continue;
-    if (a.convrot) {
-      for (int s = 1; s < 256; s *= 4) {
-        __syncthreads();
-        for (int64_t i = threadIdx.x; i < a.width / 4; i += blockDim.x) {
-          float* p = row + (i / s) * (4 * s) + i % s;
-          const float v0 = p[0], v1 = p[s], v2 = p[2 * s], v3 = p[3 * s];
-          p[0] = v0 + v1 + v2 - v3;
-          p[s] = v0 + v1 - v2 + v3;
-          p[2 * s] = v0 - v1 + v2 + v3;
-          p[3 * s] = v1 - v0 + v2 + v3;
+    if (!QUANT) continue;
+    float m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      if (a.convrot) convrot256_warp(v[c]);  // whole warps lie in the row or none of their lanes
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max_abs2_nan(m, lo2(v[c][i]), hi2(v[c][i]));
+    }
+    m = reduce.max<true>(m);
+    const bool finite = m < __uint_as_float(0x7f800000u);
+    if (!finite) {  // values that are NaN do not count for the scale
+      m = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(lo2(v[c][i])), fabsf(hi2(v[c][i]))));
+      m = reduce.max<false>(m);
+    }
+    const float scale = row_scale_from_max(m);
+    const float inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint32_t code[8];
+      if (finite) {
+        // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
+        // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 t = fma2(v[c][i], dup2(inv), dup2(12582912.0f));
+          code[i] = __float_as_uint(lo2(t));
+          code[i + 4] = __float_as_uint(hi2(t));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          code[i] = any_code(lo2(v[c][i]), scale);
+          code[i + 4] = any_code(hi2(v[c][i]), scale);
         }
       }
-      __syncthreads();
-      for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x) row[c] *= 0.0625f;
+      int8_t* q = a.q + base;
+      if (VEC) {
+        uint2 packed;
+        packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+        packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+        if (in_row[c]) *reinterpret_cast<uint2*>(q + d.at(c, 0)) = packed;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (d.at(c, j) < d.width) q[d.at(c, j)] = (int8_t)code[j];
+      }
     }
-    float m = 0.0f;
-    for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x) m = fmaxf(m, fabsf(row[c]));
-    const float scale = row_scale_from_max(norm_block_max(m, red));
-    const float inv = __fdiv_rn(1.0f, scale);
-    for (int64_t c = threadIdx.x; c < a.width; c += blockDim.x)
-      a.q[base + c] = quantize_code_rn(row[c], scale, inv);
-    if (threadIdx.x == 0) a.row_scale[r] = scale;
+    if (threadIdx.x == 0) a.row_scale[row] = scale;
   }
+  if (kRing) cp_async_wait<0>();
 }
 
-template <typename XT, typename BT>
-int launch_residual_norm(const ResidualNorm& a, cudaStream_t stream) {
-  const size_t smem = (size_t)a.width * sizeof(float);
-  auto kern = residual_norm_kernel<XT, BT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess) {
+template <typename XT, typename BT, int NC, bool VEC, bool QUANT, int SLOTS>
+int launch_norm(const ResidualNorm& a, const Deal& d, int threads, int ctas, int dev, cudaStream_t stream) {
+  auto kern = residual_norm_kernel<XT, BT, NC, VEC, QUANT, SLOTS>;
+  const size_t smem = VEC && NC == 1 ? (size_t)SLOTS * threads * 8 * (sizeof(XT) + sizeof(BT)) : 0;
+  if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     cudaGetLastError();
     return H3_ERR_CUDA;
   }
-  kern<<<(int)std::min<int64_t>(a.rows, 1 << 20), 256, smem, stream>>>(a);
+  const int grid = (int)std::min<int64_t>(a.rows, (int64_t)h3host::sm_count(dev) * ctas);
+  kern<<<grid, threads, smem, stream>>>(a, d);
   return h3host::check_launch();
+}
+
+template <typename XT, typename BT, bool QUANT>
+int launch_norm_shape(const ResidualNorm& a, bool vec, int dev, cudaStream_t stream) {
+  const int width = (int)a.width;
+  const int nc = width <= 8192 ? 1 : 4;
+  const int threads = ((width + 8 * nc - 1) / (8 * nc) + 31) / 32 * 32;
+  Deal d{width, 8, 1, 8 * threads};
+  if (width % 8 != 0) d = Deal{width, 1, threads, 8 * threads};
+  // CTAs an SM: as many as its registers hold (64 a thread), at most 16
+  const int ctas = std::min(16, std::max(1, 1024 / threads));
+  if (nc == 4)
+    return vec ? launch_norm<XT, BT, 4, true, QUANT, 2>(a, d, threads, ctas, dev, stream)
+               : launch_norm<XT, BT, 4, false, QUANT, 2>(a, d, threads, ctas, dev, stream);
+  if (!vec) return launch_norm<XT, BT, 1, false, QUANT, 2>(a, d, threads, ctas, dev, stream);
+  // four slots where all CTAs' slots fit into the SM's shared memory, else two
+  const size_t slot = (size_t)threads * 8 * (sizeof(XT) + sizeof(BT));
+  if (4 * slot * ctas <= 200 * 1024)
+    return launch_norm<XT, BT, 1, true, QUANT, 4>(a, d, threads, ctas, dev, stream);
+  return launch_norm<XT, BT, 1, true, QUANT, 2>(a, d, threads, ctas, dev, stream);
+}
+
+template <typename XT, typename BT>
+int launch_residual_norm(const ResidualNorm& a, int dev, cudaStream_t stream) {
+  bool vec = a.width % 8 == 0;
+  for (const void* p : {a.x, a.branch, (const void*)a.out, (const void*)a.h, (const void*)a.q,
+                        (const void*)a.gate, (const void*)a.shift, (const void*)a.scale,
+                        (const void*)a.post_weight, (const void*)a.post_bias,
+                        (const void*)a.pre_weight, (const void*)a.pre_bias})
+    vec = vec && h3host::aligned(p, 16);
+  if (a.mod_rows > 1) vec = vec && a.gate_ld % 4 == 0 && a.shift_ld % 4 == 0 && a.scale_ld % 4 == 0;
+  return a.q != nullptr ? launch_norm_shape<XT, BT, true>(a, vec, dev, stream)
+                        : launch_norm_shape<XT, BT, false>(a, vec, dev, stream);
 }
 
 }  // namespace h3
@@ -187,14 +519,14 @@ extern "C" int h3_residual_norm(const void* x, int x_type, const void* branch, i
   cudaStream_t st = (cudaStream_t)stream;
   if (branch == nullptr) branch_type = x_type;
   if (x_type == H3_TYPE_F32 && branch_type == H3_TYPE_F32)
-    return launch_residual_norm<float, float>(a, st);
+    return launch_residual_norm<float, float>(a, dev, st);
   if (x_type == H3_TYPE_F16 && branch_type == H3_TYPE_F16)
-    return launch_residual_norm<__half, __half>(a, st);
+    return launch_residual_norm<__half, __half>(a, dev, st);
   if (x_type == H3_TYPE_F16 && branch_type == H3_TYPE_F32)
-    return launch_residual_norm<__half, float>(a, st);
+    return launch_residual_norm<__half, float>(a, dev, st);
   if (x_type == H3_TYPE_BF16 && branch_type == H3_TYPE_BF16)
-    return launch_residual_norm<__nv_bfloat16, __nv_bfloat16>(a, st);
+    return launch_residual_norm<__nv_bfloat16, __nv_bfloat16>(a, dev, st);
   if (x_type == H3_TYPE_BF16 && branch_type == H3_TYPE_F32)
-    return launch_residual_norm<__nv_bfloat16, float>(a, st);
+    return launch_residual_norm<__nv_bfloat16, float>(a, dev, st);
   return H3_ERR_INVALID;
 }

@@ -211,13 +211,6 @@ H3_DEV void lane_angles(const RopeArgs& a, int64_t token, int u, const double* t
   }
 }
 
-H3_DEV void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-H3_DEV void cp_async8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-
 // Vector form.  Loops over rounds, tensors and steps are the same for every lane of the
 // CTA, so that every lane makes every step (the shuffles need them all).
 template <typename T, bool HALF, int G>
@@ -281,7 +274,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
         if (f_round < rounds) f_open();
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    cp_async_commit();
   };
   f_open();
 #pragma unroll 1
@@ -304,7 +297,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
       T* out = reinterpret_cast<T*>(v.out) + r.token * v.out_token + (int64_t)r.part * v.out_head;
 #pragma unroll 1
       for (int h = 0; h < steps; ++h) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        cp_async_wait<kSlots - 2>();
         f32x2 x[4] = {0, 0, 0, 0};
         if (h < count) {
           Raw<T, 8> raw;
@@ -326,7 +319,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
       }
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  cp_async_wait<0>();
 }
 
 // Any alignment, any head_dim: one element at a time.
