@@ -39,39 +39,47 @@ struct ResidualNorm {
   int* err;
 };
 
-// Sum or maximum over the CTA.  `red` has two rows of 32, used in turn: one barrier a call,
-// as a row is written again only after the barrier of the call between.
+// Sum or maximum over the CTA: a tree in each warp, one value a warp through shared memory,
+// and the same tree again in every warp.  `red` has two rows of 32, used in turn: one
+// barrier a call, as a row is written again only after the barrier of the call between.
+// Lanes without a warp read zeros, which the first call finds there.
 struct BlockReduce {
   float* red;
   int turn;
 
-  H3_DEV float* publish(float v) {
+  H3_DEV BlockReduce(float* r) : red(r), turn(0) {
+    if (threadIdx.x < 64) red[threadIdx.x] = 0.0f;
+    if (blockDim.x == 32) red[threadIdx.x + 32] = 0.0f;
+    __syncthreads();
+  }
+  H3_DEV float exchange(float v) {
     float* r = red + 32 * turn;
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    return r;
+    return r[threadIdx.x & 31];
   }
-  H3_DEV float sum(float v) {
+  H3_DEV static float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (blockDim.x == 32) return v;
-    const float* r = publish(v);
-    float t = 0.0f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += r[w];
-    return t;
+    return v;
   }
-  // NAN_WINS: NaN if any value is; else values that are NaN are left out
+  H3_DEV float sum(float v) {
+    v = warp_sum(v);
+    return blockDim.x == 32 ? v : warp_sum(exchange(v));
+  }
+  // of magnitudes; NAN_WINS: NaN if any value is, else values that are NaN are left out
+  template <bool NAN_WINS>
+  H3_DEV static float warp_max(float v) {
+    float r;
+    if (NAN_WINS) asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    else asm volatile("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+  }
   template <bool NAN_WINS>
   H3_DEV float max(float v) {
-    const auto larger = [](float a, float b) { return NAN_WINS ? max_abs2_nan(0.0f, a, b) : fmaxf(a, b); };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = larger(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (blockDim.x == 32) return v;
-    const float* r = publish(v);
-    float t = 0.0f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t = larger(t, r[w]);
-    return t;
+    v = warp_max<NAN_WINS>(v);
+    return blockDim.x == 32 ? v : warp_max<NAN_WINS>(exchange(v));
   }
 };
 
@@ -225,6 +233,16 @@ H3_DEV void load_factors(const ResidualNorm& a, const Deal& d, int chunk, bool i
   }
 }
 
+// v += gate * post bias.
+template <bool VEC>
+H3_DEV void add_post_bias(const ResidualNorm& a, const Deal& d, int chunk, bool in_row, int64_t lab, f32x2 (&v)[4]) {
+  f32x2 b[4], g[4] = {dup2(1.0f), dup2(1.0f), dup2(1.0f), dup2(1.0f)};
+  load_table<VEC>(a.post_bias, d, chunk, in_row, 0.0f, b);
+  if (a.gate != nullptr) load_table<VEC>(a.gate + lab * a.gate_ld, d, chunk, in_row, 0.0f, g);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = fma2(g[i], b[i], v[i]);
+}
+
 // (v - mean) * inv of a row, in place; values outside the row are 0 before and after.  The
 // variance of LayerNorm is taken around the mean, in a second sum.
 template <int NC, bool VEC>
@@ -267,187 +285,227 @@ __device__ __noinline__ uint32_t any_code(float v, float scale) {
   return (uint32_t)(int)quantize_code(v, scale, 0);
 }
 
-// NC chunks of eight values a thread.  NC 1: the factors stay in registers, and (VEC) rows
-// are fetched SLOTS - 1 ahead.
-template <typename XT, typename BT, int NC, bool VEC, bool QUANT, int SLOTS>
+// h of a row to its INT8 codes and row scale.
+template <int NC, bool VEC>
+H3_DEV void quantise(f32x2 (&v)[NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
+                     int64_t row, int8_t* q, BlockReduce& reduce) {
+  float m = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    if (a.convrot) convrot256_warp(v[c]);  // whole warps lie in the row or none of their lanes
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max_abs2_nan(m, lo2(v[c][i]), hi2(v[c][i]));
+  }
+  m = reduce.max<true>(m);
+  const bool finite = m < __uint_as_float(0x7f800000u);
+  if (!finite) {  // values that are NaN do not count for the scale
+    m = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(lo2(v[c][i])), fabsf(hi2(v[c][i]))));
+    m = reduce.max<false>(m);
+  }
+  const float scale = row_scale_from_max(m);
+  const float inv = __fdiv_rn(1.0f, scale);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    uint32_t code[8];
+    if (finite) {
+      // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
+      // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 t = fma2(v[c][i], dup2(inv), dup2(12582912.0f));
+        code[i] = __float_as_uint(lo2(t));
+        code[i + 4] = __float_as_uint(hi2(t));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        code[i] = any_code(lo2(v[c][i]), scale);
+        code[i + 4] = any_code(hi2(v[c][i]), scale);
+      }
+    }
+    if (VEC) {
+      uint2 packed;
+      packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+      packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+      if (in_row[c]) *reinterpret_cast<uint2*>(q + d.at(c, 0)) = packed;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (d.at(c, j) < d.width) q[d.at(c, j)] = (int8_t)code[j];
+    }
+  }
+  if (threadIdx.x == 0) a.row_scale[row] = scale;
+}
+
+H3_DEV int64_t row_label(const ResidualNorm& a, int64_t lab) {
+  if (lab >= 0 && lab < a.mod_rows) return lab;
+  report_error(a.err, H3_ERR_INVALID);
+  return 0;
+}
+
+// Rows of whole 16-byte words, one chunk a thread: factors in registers, rows fetched
+// SLOTS - 1 ahead.
+template <typename XT, typename BT, bool QUANT, int SLOTS>
 __global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ ResidualNorm a,
-                                                             const Deal d) {
+                                                             const __grid_constant__ Deal d) {
   extern __shared__ __align__(16) uint8_t slots[];
   __shared__ float red[64];
-  constexpr bool kRing = VEC && NC == 1;
   constexpr int kWordsX = sizeof(XT) / 2, kWordsB = sizeof(BT) / 2;  // 16-byte words of a chunk
-  BlockReduce reduce{red, 0};
-  bool in_row[NC];
-#pragma unroll
-  for (int c = 0; c < NC; ++c) in_row[c] = d.at(c, 0) < d.width;
+  BlockReduce reduce(red);
+  const bool in_row[1] = {(int)threadIdx.x * 8 < d.width};
   const bool branched = a.branch != nullptr;
 
   // a slot: the words of x, then of the branch, each a word a thread side by side
   const uint32_t word = blockDim.x * 16, slot_bytes = word * (kWordsX + kWordsB);
-  const uint32_t mine = kRing ? (uint32_t)__cvta_generic_to_shared(slots) + threadIdx.x * 16 : 0;
-  const auto fetch = [&](int64_t row, int slot) {
-    if (row < a.rows && in_row[0]) {
-      const uint32_t dst = mine + slot * slot_bytes;
-      const XT* x = reinterpret_cast<const XT*>(a.x) + row * a.width + d.at(0, 0);
+  uint8_t* const mine = slots + threadIdx.x * 16;
+  if (!in_row[0]) {  // values behind the row's end: zeros, never written again
 #pragma unroll
-      for (int w = 0; w < kWordsX; ++w) cp_async16(dst + w * word, x + w * (16 / sizeof(XT)));
+    for (int i = 0; i < SLOTS * (kWordsX + kWordsB); ++i)
+      *reinterpret_cast<uint4*>(mine + i * word) = make_uint4(0, 0, 0, 0);
+  }
+  const int64_t stride = gridDim.x * (int64_t)d.width, first = blockIdx.x * (int64_t)d.width + threadIdx.x * 8;
+  const XT* x_next = reinterpret_cast<const XT*>(a.x) + first;
+  const BT* b_next = reinterpret_cast<const BT*>(a.branch) + first;
+  int64_t next = blockIdx.x;
+  const auto fetch = [&](uint32_t offset) {
+    if (next < a.rows && in_row[0]) {
+      const uint32_t dst = (uint32_t)__cvta_generic_to_shared(mine) + offset;
+#pragma unroll
+      for (int w = 0; w < kWordsX; ++w) cp_async16(dst + w * word, x_next + w * (16 / sizeof(XT)));
       if (branched) {
-        const BT* b = reinterpret_cast<const BT*>(a.branch) + row * a.width + d.at(0, 0);
 #pragma unroll
         for (int w = 0; w < kWordsB; ++w)
-          cp_async16(dst + (kWordsX + w) * word, b + w * (16 / sizeof(BT)));
+          cp_async16(dst + (kWordsX + w) * word, b_next + w * (16 / sizeof(BT)));
       }
     }
+    next += gridDim.x;
+    x_next += stride;
+    b_next += stride;
     cp_async_commit();
   };
-  if (kRing) {
 #pragma unroll
-    for (int i = 0; i < SLOTS - 1; ++i) fetch(blockIdx.x + (int64_t)i * gridDim.x, i);
-  }
+  for (int i = 0; i < SLOTS - 1; ++i) fetch(i * slot_bytes);
 
   Factors f;
   int64_t held = -1;
-  int slot = 0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    int64_t lab = a.labels != nullptr ? (int64_t)__ldg(a.labels + row) : 0;
-    if (lab < 0 || lab >= a.mod_rows) {
-      report_error(a.err, H3_ERR_INVALID);
-      lab = 0;
-    }
-    if (NC == 1 && lab != held) {
-      load_factors<VEC>(a, d, 0, in_row[0], lab, f);
+  int lab_next = a.labels != nullptr && (int64_t)blockIdx.x < a.rows ? __ldg(a.labels + blockIdx.x) : 0;
+  uint32_t at = 0, refill = (SLOTS - 1) * slot_bytes;
+  int64_t offset = first;  // of this thread's values in x, out, h and q
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, offset += stride) {
+    const int64_t lab = row_label(a, lab_next);
+    if (a.labels != nullptr && row + gridDim.x < a.rows) lab_next = __ldg(a.labels + row + gridDim.x);
+    if (lab != held) {
+      load_factors<true>(a, d, 0, in_row[0], lab, f);
       held = lab;
     }
-    const int64_t base = row * a.width;
-    const uint8_t* p = slots + slot * slot_bytes + threadIdx.x * 16;
-    const auto from_slot = [&](auto type, int first, f32x2 (&v)[4]) {
+    const auto from_slot = [&](auto type, int word0, f32x2 (&v)[4]) {
       using T = decltype(type);
       Raw<T, 8> r;
       float t[8];
 #pragma unroll
       for (int w = 0; w < (int)sizeof(T) / 2; ++w)
-        *reinterpret_cast<uint4*>(&r.w[4 * w]) = *reinterpret_cast<const uint4*>(p + (first + w) * word);
+        *reinterpret_cast<uint4*>(&r.w[4 * w]) = *reinterpret_cast<const uint4*>(mine + at + (word0 + w) * word);
       r.unpack(t);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = in_row[0] ? pk2(t[i], t[i + 4]) : 0;
+      for (int i = 0; i < 4; ++i) v[i] = pk2(t[i], t[i + 4]);
     };
-    if constexpr (kRing) cp_async_wait<SLOTS - 2>();
-    f32x2 v[NC][4];  // the branch, then x', then h
+    cp_async_wait<SLOTS - 2>();
+    f32x2 v[1][4];  // the branch, then x', then h
     if (branched) {
+      from_slot(BT(), kWordsX, v[0]);
+      if (a.post_kind != H3_NORM_NONE)
+        normalise<1, true>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
+      const f32x2 rs = dup2(a.residual_scale);
+      f32x2 x[4];
+      from_slot(XT(), 0, x);
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if constexpr (kRing) from_slot(BT(), kWordsX, v[0]);
-        else load_chunk<BT, VEC>(reinterpret_cast<const BT*>(a.branch) + base, d, c, in_row[c], v[c]);
+      for (int i = 0; i < 4; ++i) v[0][i] = fma2(f.gate[i], v[0][i], mul2(x[i], rs));
+      if (a.post_bias != nullptr) add_post_bias<true>(a, d, 0, in_row[0], lab, v[0]);
+      if (in_row[0]) {
+        Raw<XT, 8> r;
+        float t[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { t[i] = lo2(v[0][i]); t[i + 4] = hi2(v[0][i]); }
+        r.pack(t);
+        r.store(reinterpret_cast<XT*>(a.out) + offset);
       }
+    } else {
+      from_slot(XT(), 0, v[0]);
+    }
+    // the slot of the row before, whose values were used up there
+    fetch(refill);
+    refill = at;
+    at = at + slot_bytes == SLOTS * slot_bytes ? 0 : at + slot_bytes;
+    if (a.pre_kind == H3_NORM_NONE) continue;
+    normalise<1, true>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[0][i] = fma2(v[0][i], f.scale[i], f.shift[i]);
+    if constexpr (QUANT) {
+      quantise<1, true>(v, a, d, in_row, row, a.q + (offset - threadIdx.x * 8), reduce);
+    } else if (in_row[0]) {
+      Raw<XT, 8> r;
+      float t[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { t[i] = lo2(v[0][i]); t[i + 4] = hi2(v[0][i]); }
+      r.pack(t);
+      r.store(reinterpret_cast<XT*>(a.h) + offset);
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// Wide rows (NC chunks a thread) and rows of any width and alignment (VEC false).
+template <typename XT, typename BT, int NC, bool VEC, bool QUANT>
+__global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_constant__ ResidualNorm a,
+                                                                 const __grid_constant__ Deal d) {
+  __shared__ float red[64];
+  BlockReduce reduce(red);
+  bool in_row[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) in_row[c] = d.at(c, 0) < d.width;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t lab = row_label(a, a.labels != nullptr ? __ldg(a.labels + row) : 0);
+    const int64_t base = row * a.width;
+    f32x2 v[NC][4];  // the branch, then x', then h
+    if (a.branch != nullptr) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        load_chunk<BT, VEC>(reinterpret_cast<const BT*>(a.branch) + base, d, c, in_row[c], v[c]);
       if (a.post_kind != H3_NORM_NONE)
         normalise<NC, VEC>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
       const f32x2 rs = dup2(a.residual_scale);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         f32x2 x[4];
-        if constexpr (kRing) from_slot(XT(), 0, x);
-        else load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], x);
-        if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
+        load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], x);
+        Factors f;
+        load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[c][i] = fma2(f.gate[i], v[c][i], mul2(x[i], rs));
-        if (a.post_bias != nullptr) {  // + gate * bias
-          f32x2 b[4], g[4] = {dup2(1.0f), dup2(1.0f), dup2(1.0f), dup2(1.0f)};
-          load_table<VEC>(a.post_bias, d, c, in_row[c], 0.0f, b);
-          if (a.gate != nullptr) load_table<VEC>(a.gate + lab * a.gate_ld, d, c, in_row[c], 0.0f, g);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[c][i] = fma2(g[i], b[i], v[c][i]);
-        }
+        if (a.post_bias != nullptr) add_post_bias<VEC>(a, d, c, in_row[c], lab, v[c]);
         store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.out) + base, d, c, in_row[c], v[c]);
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if constexpr (kRing) from_slot(XT(), 0, v[0]);
-        else load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], v[c]);
-      }
-    }
-    if constexpr (kRing) {
-      // the slot of the row before, whose values were used up there
-      fetch(row + (int64_t)(SLOTS - 1) * gridDim.x, slot == 0 ? SLOTS - 1 : slot - 1);
-      slot = slot + 1 == SLOTS ? 0 : slot + 1;
+      for (int c = 0; c < NC; ++c)
+        load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], v[c]);
     }
     if (a.pre_kind == H3_NORM_NONE) continue;
     normalise<NC, VEC>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
+      Factors f;
+      load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], f.scale[i], f.shift[i]);
       if (!QUANT) store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.h) + base, d, c, in_row[c], v[c]);
     }
-    if (!QUANT) continue;
-    float m = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      if (a.convrot) convrot256_warp(v[c]);  // whole warps lie in the row or none of their lanes
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = max_abs2_nan(m, lo2(v[c][i]), hi2(v[c][i]));
-    }
-    m = reduce.max<true>(m);
-    const bool finite = m < __uint_as_float(0x7f800000u);
-    if (!finite) {  // values that are NaN do not count for the scale
-      m = 0.0f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(lo2(v[c][i])), fabsf(hi2(v[c][i]))));
-      m = reduce.max<false>(m);
-    }
-    const float scale = row_scale_from_max(m);
-    const float inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint32_t code[8];
-      if (finite) {
-        // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
-        // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x2 t = fma2(v[c][i], dup2(inv), dup2(12582912.0f));
-          code[i] = __float_as_uint(lo2(t));
-          code[i + 4] = __float_as_uint(hi2(t));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          code[i] = any_code(lo2(v[c][i]), scale);
-          code[i + 4] = any_code(hi2(v[c][i]), scale);
-        }
-      }
-      int8_t* q = a.q + base;
-      if (VEC) {
-        uint2 packed;
-        packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
-        packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
-        if (in_row[c]) *reinterpret_cast<uint2*>(q + d.at(c, 0)) = packed;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (d.at(c, j) < d.width) q[d.at(c, j)] = (int8_t)code[j];
-      }
-    }
-    if (threadIdx.x == 0) a.row_scale[row] = scale;
+    if (QUANT) quantise<NC, VEC>(v, a, d, in_row, row, a.q + base, reduce);
   }
-  if (kRing) cp_async_wait<0>();
-}
-
-template <typename XT, typename BT, int NC, bool VEC, bool QUANT, int SLOTS>
-int launch_norm(const ResidualNorm& a, const Deal& d, int threads, int ctas, int dev, cudaStream_t stream) {
-  auto kern = residual_norm_kernel<XT, BT, NC, VEC, QUANT, SLOTS>;
-  const size_t smem = VEC && NC == 1 ? (size_t)SLOTS * threads * 8 * (sizeof(XT) + sizeof(BT)) : 0;
-  if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
-    return H3_ERR_CUDA;
-  }
-  const int grid = (int)std::min<int64_t>(a.rows, (int64_t)h3host::sm_count(dev) * ctas);
-  kern<<<grid, threads, smem, stream>>>(a, d);
-  return h3host::check_launch();
 }
 
 template <typename XT, typename BT, bool QUANT>
@@ -459,15 +517,26 @@ int launch_norm_shape(const ResidualNorm& a, bool vec, int dev, cudaStream_t str
   if (width % 8 != 0) d = Deal{width, 1, threads, 8 * threads};
   // CTAs an SM: as many as its registers hold (64 a thread), at most 16
   const int ctas = std::min(16, std::max(1, 1024 / threads));
-  if (nc == 4)
-    return vec ? launch_norm<XT, BT, 4, true, QUANT, 2>(a, d, threads, ctas, dev, stream)
-               : launch_norm<XT, BT, 4, false, QUANT, 2>(a, d, threads, ctas, dev, stream);
-  if (!vec) return launch_norm<XT, BT, 1, false, QUANT, 2>(a, d, threads, ctas, dev, stream);
-  // four slots where all CTAs' slots fit into the SM's shared memory, else two
-  const size_t slot = (size_t)threads * 8 * (sizeof(XT) + sizeof(BT));
-  if (4 * slot * ctas <= 200 * 1024)
-    return launch_norm<XT, BT, 1, true, QUANT, 4>(a, d, threads, ctas, dev, stream);
-  return launch_norm<XT, BT, 1, true, QUANT, 2>(a, d, threads, ctas, dev, stream);
+  const int grid = (int)std::min<int64_t>(a.rows, (int64_t)h3host::sm_count(dev) * ctas);
+  if (nc == 4) {
+    if (vec) residual_norm_any_kernel<XT, BT, 4, true, QUANT><<<grid, threads, 0, stream>>>(a, d);
+    else residual_norm_any_kernel<XT, BT, 4, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
+  } else if (!vec) {
+    residual_norm_any_kernel<XT, BT, 1, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
+  } else {
+    // four slots where all CTAs' slots fit into the SM's shared memory, else two
+    const size_t slot = (size_t)threads * 8 * (sizeof(XT) + sizeof(BT));
+    const bool four = 4 * slot * ctas <= 200 * 1024;
+    auto kern = four ? residual_norm_kernel<XT, BT, QUANT, 4> : residual_norm_kernel<XT, BT, QUANT, 2>;
+    const size_t smem = slot * (four ? 4 : 2);
+    if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+      cudaGetLastError();
+      return H3_ERR_CUDA;
+    }
+    kern<<<grid, threads, smem, stream>>>(a, d);
+  }
+  return h3host::check_launch();
 }
 
 template <typename XT, typename BT>
