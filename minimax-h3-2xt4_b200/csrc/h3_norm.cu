@@ -16,6 +16,8 @@
 
 namespace h3 {
 
+constexpr int kPairThreads = 768;  // most threads of a CTA that takes two rows: 80 registers each
+
 struct ResidualNorm {
   const void* x;
   const void* branch;
@@ -39,34 +41,53 @@ struct ResidualNorm {
   int* err;
 };
 
-// Sum or maximum over the CTA: a tree in each warp, one value a warp through shared memory,
-// and the same tree again in every warp.  `red` has two rows of 32, used in turn: one
-// barrier a call, as a row is written again only after the barrier of the call between.
-// Lanes without a warp read zeros, which the first call finds there.
+// Sums or maxima over the CTA, of one row or of two at once: a tree in each warp, one value
+// a warp through shared memory, and the same tree again in every warp.  The trees add in
+// one order, whether a row is reduced alone or with another.  `red` has two blocks of 64,
+// used in turn: one barrier a call, as a block is written again only after the barrier of
+// the call between.  Places without a warp hold zeros from the start.
+template <int ROWS>
 struct BlockReduce {
   float* red;
   int turn;
 
   H3_DEV BlockReduce(float* r) : red(r), turn(0) {
-    if (threadIdx.x < 64) red[threadIdx.x] = 0.0f;
-    if (blockDim.x == 32) red[threadIdx.x + 32] = 0.0f;
+    for (int i = threadIdx.x; i < 128; i += blockDim.x) red[i] = 0.0f;
     __syncthreads();
   }
-  H3_DEV float exchange(float v) {
-    float* r = red + 32 * turn;
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return r[threadIdx.x & 31];
+  // value of warp w, row r at [w & 15][w >> 4][r]
+  H3_DEV float* next() {
+    turn ^= 64;
+    return red + turn;
   }
-  H3_DEV static float warp_sum(float v) {
+  H3_DEV static int place(int warp) { return (warp & 15) * 4 + (warp >> 4) * 2; }
+
+  H3_DEV void sum(float (&v)[ROWS]) {
+    const int lane = threadIdx.x & 31;
+    float t;
+    if (ROWS == 1) {
+      t = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+    } else {  // the lower lanes go on with the first row, the upper ones with the second
+      t = lane < 16 ? v[0] : v[ROWS - 1];
+      t += __shfl_xor_sync(0xffffffffu, lane < 16 ? v[ROWS - 1] : v[0], 16);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  }
-  H3_DEV float sum(float v) {
-    v = warp_sum(v);
-    return blockDim.x == 32 ? v : warp_sum(exchange(v));
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (blockDim.x > 32) {
+      float* r = next();
+      if ((lane & 15) == 0 && (ROWS == 2 || lane == 0)) r[place(threadIdx.x >> 5) + (lane >> 4)] = t;
+      __syncthreads();
+      const float* mine = r + (lane & 15) * 4 + (ROWS == 2 ? lane >> 4 : 0);
+      t = mine[0] + mine[2];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (ROWS == 1) {
+      v[0] = t;
+    } else {
+      v[0] = __shfl_sync(0xffffffffu, t, 0);
+      v[ROWS - 1] = __shfl_sync(0xffffffffu, t, 16);
+    }
   }
   // of magnitudes; NAN_WINS: NaN if any value is, else values that are NaN are left out
   template <bool NAN_WINS>
@@ -77,9 +98,16 @@ struct BlockReduce {
     return r;
   }
   template <bool NAN_WINS>
-  H3_DEV float max(float v) {
-    v = warp_max<NAN_WINS>(v);
-    return blockDim.x == 32 ? v : warp_max<NAN_WINS>(exchange(v));
+  H3_DEV void max(float (&v)[ROWS]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) v[i] = warp_max<NAN_WINS>(v[i]);
+    if (blockDim.x == 32) return;
+    float* r = next();
+    if (lane < ROWS) r[place(threadIdx.x >> 5) + lane] = v[lane == 0 ? 0 : ROWS - 1];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) v[i] = warp_max<NAN_WINS>(r[lane * 2 + i]);
   }
 };
 
@@ -243,40 +271,57 @@ H3_DEV void add_post_bias(const ResidualNorm& a, const Deal& d, int chunk, bool 
   for (int i = 0; i < 4; ++i) v[i] = fma2(g[i], b[i], v[i]);
 }
 
-// (v - mean) * inv of a row, in place; values outside the row are 0 before and after.  The
-// variance of LayerNorm is taken around the mean, in a second sum.
-template <int NC, bool VEC>
-H3_DEV void normalise(f32x2 (&v)[NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
-                      int kind, float eps, BlockReduce& reduce) {
+// (v - mean) * inv of ROWS rows, in place; values outside the row are 0 before and after.
+// The variance of LayerNorm is taken around the mean, in a second sum.
+template <int ROWS, int NC, bool VEC>
+H3_DEV void normalise(f32x2 (&v)[ROWS][NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
+                      int kind, float eps, BlockReduce<ROWS>& reduce) {
+  float sum[ROWS];
   if (kind == H3_NORM_LAYER) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      f32x2 t = 0;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t = add2(t, v[r][c][i]);
+      sum[r] = lo2(t) + hi2(t);
+    }
+    reduce.sum(sum);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const f32x2 mean = dup2(sum[r] * a.inv_width);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 m = sub2(v[r][c][i], mean);
+          if (VEC) {
+            v[r][c][i] = in_row[c] ? m : 0;
+          } else {
+            v[r][c][i] = pk2(d.at(c, i) < d.width ? lo2(m) : 0.0f, d.at(c, i + 4) < d.width ? hi2(m) : 0.0f);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
     f32x2 t = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t = add2(t, v[c][i]);
-    const f32x2 mean = dup2(reduce.sum(lo2(t) + hi2(t)) * a.inv_width);
+      for (int i = 0; i < 4; ++i) t = fma2(v[r][c][i], v[r][c][i], t);
+    sum[r] = lo2(t) + hi2(t);
+  }
+  reduce.sum(sum);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const f32x2 inv = dup2(rsqrtf(__fmaf_rn(sum[r], a.inv_width, eps)));
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x2 m = sub2(v[c][i], mean);
-        if (VEC) {
-          v[c][i] = in_row[c] ? m : 0;
-        } else {
-          v[c][i] = pk2(d.at(c, i) < d.width ? lo2(m) : 0.0f, d.at(c, i + 4) < d.width ? hi2(m) : 0.0f);
-        }
-      }
+      for (int i = 0; i < 4; ++i) v[r][c][i] = mul2(v[r][c][i], inv);
   }
-  f32x2 t = 0;
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t = fma2(v[c][i], v[c][i], t);
-  const f32x2 inv = dup2(rsqrtf(__fmaf_rn(reduce.sum(lo2(t) + hi2(t)), a.inv_width, eps)));
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[c][i] = mul2(v[c][i], inv);
 }
 
 // The code of a value of a row that holds infinities or NaN (rare: kept out of line, where
@@ -285,60 +330,77 @@ __device__ __noinline__ uint32_t any_code(float v, float scale) {
   return (uint32_t)(int)quantize_code(v, scale, 0);
 }
 
-// h of a row to its INT8 codes and row scale.
-template <int NC, bool VEC>
-H3_DEV void quantise(f32x2 (&v)[NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
-                     int64_t row, int8_t* q, BlockReduce& reduce) {
-  float m = 0.0f;
+// h of ROWS rows to their INT8 codes and row scales; rows outside `todo` are not stored.
+template <int ROWS, int NC, bool VEC>
+H3_DEV void quantise(f32x2 (&v)[ROWS][NC][4], const ResidualNorm& a, const Deal& d, const bool (&in_row)[NC],
+                     int64_t row, uint32_t todo, BlockReduce<ROWS>& reduce) {
+  float m[ROWS];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    if (a.convrot) convrot256_warp(v[c]);  // whole warps lie in the row or none of their lanes
+  for (int r = 0; r < ROWS; ++r) {
+    m[r] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max_abs2_nan(m, lo2(v[c][i]), hi2(v[c][i]));
-  }
-  m = reduce.max<true>(m);
-  const bool finite = m < __uint_as_float(0x7f800000u);
-  if (!finite) {  // values that are NaN do not count for the scale
-    m = 0.0f;
+    for (int c = 0; c < NC; ++c) {
+      if (a.convrot) convrot256_warp(v[r][c]);  // whole warps lie in the row or none of their lanes
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(lo2(v[c][i])), fabsf(hi2(v[c][i]))));
-    m = reduce.max<false>(m);
-  }
-  const float scale = row_scale_from_max(m);
-  const float inv = __fdiv_rn(1.0f, scale);
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    uint32_t code[8];
-    if (finite) {
-      // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
-      // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x2 t = fma2(v[c][i], dup2(inv), dup2(12582912.0f));
-        code[i] = __float_as_uint(lo2(t));
-        code[i + 4] = __float_as_uint(hi2(t));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        code[i] = any_code(lo2(v[c][i]), scale);
-        code[i + 4] = any_code(hi2(v[c][i]), scale);
-      }
-    }
-    if (VEC) {
-      uint2 packed;
-      packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
-      packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
-      if (in_row[c]) *reinterpret_cast<uint2*>(q + d.at(c, 0)) = packed;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (d.at(c, j) < d.width) q[d.at(c, j)] = (int8_t)code[j];
+      for (int i = 0; i < 4; ++i) m[r] = max_abs2_nan(m[r], lo2(v[r][c][i]), hi2(v[r][c][i]));
     }
   }
-  if (threadIdx.x == 0) a.row_scale[row] = scale;
+  reduce.template max<true>(m);
+  bool finite[ROWS], all_finite = true;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    finite[r] = m[r] < __uint_as_float(0x7f800000u);
+    all_finite = all_finite && finite[r];
+  }
+  if (!all_finite) {  // values that are NaN do not count for the scale
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      m[r] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[r] = fmaxf(m[r], fmaxf(fabsf(lo2(v[r][c][i])), fabsf(hi2(v[r][c][i]))));
+    }
+    reduce.template max<false>(m);
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const float scale = row_scale_from_max(m[r]);
+    const float inv = __fdiv_rn(1.0f, scale);
+    int8_t* q = a.q + (row + r) * d.width;
+    if (!(todo >> r & 1)) continue;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint32_t code[8];
+      if (finite[r]) {
+        // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
+        // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x2 t = fma2(v[r][c][i], dup2(inv), dup2(12582912.0f));
+          code[i] = __float_as_uint(lo2(t));
+          code[i + 4] = __float_as_uint(hi2(t));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          code[i] = any_code(lo2(v[r][c][i]), scale);
+          code[i + 4] = any_code(hi2(v[r][c][i]), scale);
+        }
+      }
+      if (VEC) {
+        uint2 packed;
+        packed.x = __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410);
+        packed.y = __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410);
+        if (in_row[c]) *reinterpret_cast<uint2*>(q + d.at(c, 0)) = packed;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (d.at(c, j) < d.width) q[d.at(c, j)] = (int8_t)code[j];
+      }
+    }
+    if (threadIdx.x == 0) a.row_scale[row + r] = scale;
+  }
 }
 
 H3_DEV int64_t row_label(const ResidualNorm& a, int64_t lab) {
@@ -347,113 +409,140 @@ H3_DEV int64_t row_label(const ResidualNorm& a, int64_t lab) {
   return 0;
 }
 
-// Rows of whole 16-byte words, one chunk a thread: factors in registers, rows fetched
-// SLOTS - 1 ahead.
-template <typename XT, typename BT, bool QUANT, int SLOTS>
-__global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_constant__ ResidualNorm a,
-                                                             const __grid_constant__ Deal d) {
-  extern __shared__ __align__(16) uint8_t slots[];
-  __shared__ float red[64];
-  constexpr int kWordsX = sizeof(XT) / 2, kWordsB = sizeof(BT) / 2;  // 16-byte words of a chunk
-  BlockReduce reduce(red);
-  const bool in_row[1] = {(int)threadIdx.x * 8 < d.width};
-  const bool branched = a.branch != nullptr;
+// A chunk of fp32 pairs to memory in its type.
+template <typename T>
+H3_DEV void store_pairs(T* p, const f32x2 (&v)[4]) {
+  Raw<T, 8> r;
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = lo2(v[i]);
+    t[i + 4] = hi2(v[i]);
+  }
+  r.pack(t);
+  r.store(p);
+}
 
-  // a slot: the words of x, then of the branch, each a word a thread side by side
-  const uint32_t word = blockDim.x * 16, slot_bytes = word * (kWordsX + kWordsB);
+// Rows of whole 16-byte words, one chunk a thread, ROWS neighbouring rows at a time: two
+// share their reductions, addresses and barriers (a third of all instructions) and cover
+// each other's latencies.  Factors stay in registers, row groups are fetched SLOTS - 1 ahead.
+template <typename XT, typename BT, bool BRANCH, bool QUANT, int ROWS, int SLOTS>
+__global__ void __launch_bounds__(ROWS == 1 ? 1024 : kPairThreads)
+    residual_norm_kernel(const __grid_constant__ ResidualNorm a, const __grid_constant__ Deal d) {
+  extern __shared__ __align__(16) uint8_t slots[];
+  __shared__ float red[128];
+  constexpr int kWordsX = sizeof(XT) / 2, kWordsB = BRANCH ? sizeof(BT) / 2 : 0;  // 16-byte words of a chunk
+  constexpr int kWords = ROWS * (kWordsX + kWordsB);
+  BlockReduce<ROWS> reduce(red);
+  const bool in_row[1] = {(int)threadIdx.x * 8 < d.width};
+
+  // a slot: for each row the words of x, then of the branch, each a word a thread side by side
+  const uint32_t word = blockDim.x * 16, slot_bytes = word * kWords;
   uint8_t* const mine = slots + threadIdx.x * 16;
   if (!in_row[0]) {  // values behind the row's end: zeros, never written again
 #pragma unroll
-    for (int i = 0; i < SLOTS * (kWordsX + kWordsB); ++i)
+    for (int i = 0; i < SLOTS * kWords; ++i)
       *reinterpret_cast<uint4*>(mine + i * word) = make_uint4(0, 0, 0, 0);
   }
-  const int64_t stride = gridDim.x * (int64_t)d.width, first = blockIdx.x * (int64_t)d.width + threadIdx.x * 8;
+  const int64_t step = (int64_t)gridDim.x * ROWS, stride = step * d.width;
+  const int64_t first = (int64_t)blockIdx.x * ROWS * d.width + threadIdx.x * 8;
   const XT* x_next = reinterpret_cast<const XT*>(a.x) + first;
   const BT* b_next = reinterpret_cast<const BT*>(a.branch) + first;
-  int64_t next = blockIdx.x;
+  int64_t next = (int64_t)blockIdx.x * ROWS;
   const auto fetch = [&](uint32_t offset) {
-    if (next < a.rows && in_row[0]) {
+    if (in_row[0]) {
       const uint32_t dst = (uint32_t)__cvta_generic_to_shared(mine) + offset;
 #pragma unroll
-      for (int w = 0; w < kWordsX; ++w) cp_async16(dst + w * word, x_next + w * (16 / sizeof(XT)));
-      if (branched) {
+      for (int r = 0; r < ROWS; ++r) {
+        if (next + r >= a.rows) break;
+#pragma unroll
+        for (int w = 0; w < kWordsX; ++w)
+          cp_async16(dst + (r * (kWordsX + kWordsB) + w) * word, x_next + r * d.width + w * (16 / sizeof(XT)));
 #pragma unroll
         for (int w = 0; w < kWordsB; ++w)
-          cp_async16(dst + (kWordsX + w) * word, b_next + w * (16 / sizeof(BT)));
+          cp_async16(dst + (r * (kWordsX + kWordsB) + kWordsX + w) * word,
+                     b_next + r * d.width + w * (16 / sizeof(BT)));
       }
     }
-    next += gridDim.x;
+    next += step;
     x_next += stride;
-    b_next += stride;
+    if (BRANCH) b_next += stride;
     cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < SLOTS - 1; ++i) fetch(i * slot_bytes);
 
   Factors f;
-  int64_t held = -1;
-  int lab_next = a.labels != nullptr && (int64_t)blockIdx.x < a.rows ? __ldg(a.labels + blockIdx.x) : 0;
-  uint32_t at = 0, refill = (SLOTS - 1) * slot_bytes;
+  int held = -1;
+  int lab[ROWS], lab_next[ROWS];
+  const auto labels_at = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      lab_next[r] = a.labels != nullptr && row + r < a.rows ? __ldg(a.labels + row + r) : 0;
+  };
+  labels_at((int64_t)blockIdx.x * ROWS);
+  uint32_t at = 0;
   int64_t offset = first;  // of this thread's values in x, out, h and q
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, offset += stride) {
-    const int64_t lab = row_label(a, lab_next);
-    if (a.labels != nullptr && row + gridDim.x < a.rows) lab_next = __ldg(a.labels + row + gridDim.x);
-    if (lab != held) {
-      load_factors<true>(a, d, 0, in_row[0], lab, f);
-      held = lab;
-    }
+  for (int64_t row = (int64_t)blockIdx.x * ROWS; row < a.rows; row += step, offset += stride) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) lab[r] = (int)row_label(a, lab_next[r]);
+    labels_at(row + step);
     const auto from_slot = [&](auto type, int word0, f32x2 (&v)[4]) {
       using T = decltype(type);
-      Raw<T, 8> r;
+      Raw<T, 8> raw;
       float t[8];
 #pragma unroll
       for (int w = 0; w < (int)sizeof(T) / 2; ++w)
-        *reinterpret_cast<uint4*>(&r.w[4 * w]) = *reinterpret_cast<const uint4*>(mine + at + (word0 + w) * word);
-      r.unpack(t);
+        *reinterpret_cast<uint4*>(&raw.w[4 * w]) = *reinterpret_cast<const uint4*>(mine + at + (word0 + w) * word);
+      raw.unpack(t);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = pk2(t[i], t[i + 4]);
     };
-    cp_async_wait<SLOTS - 2>();
-    f32x2 v[1][4];  // the branch, then x', then h
-    if (branched) {
-      from_slot(BT(), kWordsX, v[0]);
-      if (a.post_kind != H3_NORM_NONE)
-        normalise<1, true>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
-      const f32x2 rs = dup2(a.residual_scale);
-      f32x2 x[4];
-      from_slot(XT(), 0, x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[0][i] = fma2(f.gate[i], v[0][i], mul2(x[i], rs));
-      if (a.post_bias != nullptr) add_post_bias<true>(a, d, 0, in_row[0], lab, v[0]);
-      if (in_row[0]) {
-        Raw<XT, 8> r;
-        float t[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { t[i] = lo2(v[0][i]); t[i + 4] = hi2(v[0][i]); }
-        r.pack(t);
-        r.store(reinterpret_cast<XT*>(a.out) + offset);
+    // into the slot of the rows before, whose values were used up there
+    fetch(at == 0 ? (SLOTS - 1) * slot_bytes : at - slot_bytes);
+    cp_async_wait<SLOTS - 1>();
+    uint32_t todo = ROWS == 2 && row + 1 < a.rows ? 3 : 1;
+    // rows of different labels are stored one after the other, each under its own factors
+    do {
+      const int label = todo & 1 ? lab[0] : lab[ROWS - 1];
+      const uint32_t now = ROWS == 2 && todo == 3 && lab[0] != lab[ROWS - 1] ? 1 : todo;
+      todo ^= now;
+      if (label != held) {
+        load_factors<true>(a, d, 0, in_row[0], label, f);
+        held = label;
       }
-    } else {
-      from_slot(XT(), 0, v[0]);
-    }
-    // the slot of the row before, whose values were used up there
-    fetch(refill);
-    refill = at;
+      f32x2 v[ROWS][1][4];  // the branch, then x', then h
+      if constexpr (BRANCH) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) from_slot(BT(), r * (kWordsX + kWordsB) + kWordsX, v[r][0]);
+        if (a.post_kind != H3_NORM_NONE)
+          normalise<ROWS, 1, true>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
+        const f32x2 rs = dup2(a.residual_scale);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          f32x2 x[4];
+          from_slot(XT(), r * (kWordsX + kWordsB), x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[r][0][i] = fma2(f.gate[i], v[r][0][i], mul2(x[i], rs));
+          if (a.post_bias != nullptr) add_post_bias<true>(a, d, 0, in_row[0], label, v[r][0]);
+          if (in_row[0] && (now >> r & 1)) store_pairs(reinterpret_cast<XT*>(a.out) + offset + r * d.width, v[r][0]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) from_slot(XT(), r * kWordsX, v[r][0]);
+      }
+      if (a.pre_kind == H3_NORM_NONE) continue;
+      normalise<ROWS, 1, true>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[r][0][i] = fma2(v[r][0][i], f.scale[i], f.shift[i]);
+        if (!QUANT && in_row[0] && (now >> r & 1))
+          store_pairs(reinterpret_cast<XT*>(a.h) + offset + r * d.width, v[r][0]);
+      }
+      if constexpr (QUANT) quantise<ROWS, 1, true>(v, a, d, in_row, row, now, reduce);
+    } while (todo != 0);
     at = at + slot_bytes == SLOTS * slot_bytes ? 0 : at + slot_bytes;
-    if (a.pre_kind == H3_NORM_NONE) continue;
-    normalise<1, true>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[0][i] = fma2(v[0][i], f.scale[i], f.shift[i]);
-    if constexpr (QUANT) {
-      quantise<1, true>(v, a, d, in_row, row, a.q + (offset - threadIdx.x * 8), reduce);
-    } else if (in_row[0]) {
-      Raw<XT, 8> r;
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { t[i] = lo2(v[0][i]); t[i + 4] = hi2(v[0][i]); }
-      r.pack(t);
-      r.store(reinterpret_cast<XT*>(a.h) + offset);
-    }
   }
   cp_async_wait<0>();
 }
@@ -462,21 +551,21 @@ __global__ void __launch_bounds__(1024) residual_norm_kernel(const __grid_consta
 template <typename XT, typename BT, int NC, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_constant__ ResidualNorm a,
                                                                  const __grid_constant__ Deal d) {
-  __shared__ float red[64];
-  BlockReduce reduce(red);
+  __shared__ float red[128];
+  BlockReduce<1> reduce(red);
   bool in_row[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) in_row[c] = d.at(c, 0) < d.width;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t lab = row_label(a, a.labels != nullptr ? __ldg(a.labels + row) : 0);
     const int64_t base = row * a.width;
-    f32x2 v[NC][4];  // the branch, then x', then h
+    f32x2 v[1][NC][4];  // the branch, then x', then h
     if (a.branch != nullptr) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        load_chunk<BT, VEC>(reinterpret_cast<const BT*>(a.branch) + base, d, c, in_row[c], v[c]);
+        load_chunk<BT, VEC>(reinterpret_cast<const BT*>(a.branch) + base, d, c, in_row[c], v[0][c]);
       if (a.post_kind != H3_NORM_NONE)
-        normalise<NC, VEC>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
+        normalise<1, NC, VEC>(v, a, d, in_row, a.post_kind, a.post_eps, reduce);
       const f32x2 rs = dup2(a.residual_scale);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -485,57 +574,68 @@ __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_co
         Factors f;
         load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c][i] = fma2(f.gate[i], v[c][i], mul2(x[i], rs));
-        if (a.post_bias != nullptr) add_post_bias<VEC>(a, d, c, in_row[c], lab, v[c]);
-        store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.out) + base, d, c, in_row[c], v[c]);
+        for (int i = 0; i < 4; ++i) v[0][c][i] = fma2(f.gate[i], v[0][c][i], mul2(x[i], rs));
+        if (a.post_bias != nullptr) add_post_bias<VEC>(a, d, c, in_row[c], lab, v[0][c]);
+        store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.out) + base, d, c, in_row[c], v[0][c]);
       }
     } else {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], v[c]);
+        load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], v[0][c]);
     }
     if (a.pre_kind == H3_NORM_NONE) continue;
-    normalise<NC, VEC>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
+    normalise<1, NC, VEC>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       Factors f;
       load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[c][i] = fma2(v[c][i], f.scale[i], f.shift[i]);
-      if (!QUANT) store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.h) + base, d, c, in_row[c], v[c]);
+      for (int i = 0; i < 4; ++i) v[0][c][i] = fma2(v[0][c][i], f.scale[i], f.shift[i]);
+      if (!QUANT) store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.h) + base, d, c, in_row[c], v[0][c]);
     }
-    if (QUANT) quantise<NC, VEC>(v, a, d, in_row, row, a.q + base, reduce);
+    if (QUANT) quantise<1, NC, VEC>(v, a, d, in_row, row, 1, reduce);
   }
 }
 
-template <typename XT, typename BT, bool QUANT>
+template <typename XT, typename BT, bool BRANCH, bool QUANT, int ROWS, int SLOTS>
+int launch_ring(const ResidualNorm& a, const Deal& d, int threads, int dev, cudaStream_t stream) {
+  auto kern = residual_norm_kernel<XT, BT, BRANCH, QUANT, ROWS, SLOTS>;
+  const size_t smem = (size_t)SLOTS * ROWS * threads * 8 * (sizeof(XT) + (BRANCH ? sizeof(BT) : 0));
+  if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return H3_ERR_CUDA;
+  }
+  // CTAs an SM: what its registers and its shared memory hold
+  const int by_regs = 65536 / ((ROWS == 1 ? 64 : 80) * threads), by_smem = (int)(220 * 1024 / (smem + 2048));
+  const int ctas = std::max(1, std::min(std::min(by_regs, by_smem), 16));
+  const int grid = (int)std::min<int64_t>((a.rows + ROWS - 1) / ROWS, (int64_t)h3host::sm_count(dev) * ctas);
+  kern<<<grid, threads, smem, stream>>>(a, d);
+  return h3host::check_launch();
+}
+
+template <typename XT, typename BT, bool BRANCH, bool QUANT>
 int launch_norm_shape(const ResidualNorm& a, bool vec, int dev, cudaStream_t stream) {
   const int width = (int)a.width;
   const int nc = width <= 8192 ? 1 : 4;
   const int threads = ((width + 8 * nc - 1) / (8 * nc) + 31) / 32 * 32;
   Deal d{width, 8, 1, 8 * threads};
   if (width % 8 != 0) d = Deal{width, 1, threads, 8 * threads};
-  // CTAs an SM: as many as its registers hold (64 a thread), at most 16
+  if (nc == 1 && vec) {
+    // Two rows at a time where the registers allow it, there are rows for every SM to have
+    // several pairs, and three slots of a pair fit; else one row, in four slots or two.
+    const int64_t pair = 2ll * threads * 8 * (sizeof(XT) + (BRANCH ? sizeof(BT) : 0));
+    if (threads <= kPairThreads && a.rows >= 4ll * h3host::sm_count(dev) && 3 * pair <= 200 * 1024)
+      return launch_ring<XT, BT, BRANCH, QUANT, 2, 3>(a, d, threads, dev, stream);
+    if (4 * pair / 2 <= 100 * 1024)
+      return launch_ring<XT, BT, BRANCH, QUANT, 1, 4>(a, d, threads, dev, stream);
+    return launch_ring<XT, BT, BRANCH, QUANT, 1, 2>(a, d, threads, dev, stream);
+  }
   const int ctas = std::min(16, std::max(1, 1024 / threads));
   const int grid = (int)std::min<int64_t>(a.rows, (int64_t)h3host::sm_count(dev) * ctas);
-  if (nc == 4) {
-    if (vec) residual_norm_any_kernel<XT, BT, 4, true, QUANT><<<grid, threads, 0, stream>>>(a, d);
-    else residual_norm_any_kernel<XT, BT, 4, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
-  } else if (!vec) {
-    residual_norm_any_kernel<XT, BT, 1, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
-  } else {
-    // four slots where all CTAs' slots fit into the SM's shared memory, else two
-    const size_t slot = (size_t)threads * 8 * (sizeof(XT) + sizeof(BT));
-    const bool four = 4 * slot * ctas <= 200 * 1024;
-    auto kern = four ? residual_norm_kernel<XT, BT, QUANT, 4> : residual_norm_kernel<XT, BT, QUANT, 2>;
-    const size_t smem = slot * (four ? 4 : 2);
-    if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-      cudaGetLastError();
-      return H3_ERR_CUDA;
-    }
-    kern<<<grid, threads, smem, stream>>>(a, d);
-  }
+  if (nc == 1) residual_norm_any_kernel<XT, BT, 1, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
+  else if (vec) residual_norm_any_kernel<XT, BT, 4, true, QUANT><<<grid, threads, 0, stream>>>(a, d);
+  else residual_norm_any_kernel<XT, BT, 4, false, QUANT><<<grid, threads, 0, stream>>>(a, d);
   return h3host::check_launch();
 }
 
@@ -548,8 +648,12 @@ int launch_residual_norm(const ResidualNorm& a, int dev, cudaStream_t stream) {
                         (const void*)a.pre_weight, (const void*)a.pre_bias})
     vec = vec && h3host::aligned(p, 16);
   if (a.mod_rows > 1) vec = vec && a.gate_ld % 4 == 0 && a.shift_ld % 4 == 0 && a.scale_ld % 4 == 0;
-  return a.q != nullptr ? launch_norm_shape<XT, BT, true>(a, vec, dev, stream)
-                        : launch_norm_shape<XT, BT, false>(a, vec, dev, stream);
+  if constexpr (sizeof(XT) == sizeof(BT))  // without a branch both types are x's
+    if (a.branch == nullptr)
+      return a.q != nullptr ? launch_norm_shape<XT, BT, false, true>(a, vec, dev, stream)
+                            : launch_norm_shape<XT, BT, false, false>(a, vec, dev, stream);
+  return a.q != nullptr ? launch_norm_shape<XT, BT, true, true>(a, vec, dev, stream)
+                        : launch_norm_shape<XT, BT, true, false>(a, vec, dev, stream);
 }
 
 }  // namespace h3
