@@ -30,16 +30,18 @@ struct Int4Args {
   const float* bias;
   void* out;
   int groups, pitch;  // of a weight row: groups, bytes
-  int group_shift;    // log2(group) - 5
+  int scale_type, out_type;
+  int wn;             // column tiles of a CTA at a time
   int chunk;          // k of a chunk of staged x, a multiple of kStageK
-  int out_type;
+  int x_vec;          // rows of x start on 16-byte boundaries
 };
 
-constexpr int kInt4Warps = 8;
+constexpr int kInt4Warps = 16;
 constexpr int kStageK = 256;                   // k of one stage of packed weights
 constexpr int kStagePitch = kStageK / 2 + 16;  // bytes of a stage's row: the eight rows that a
                                                // load touches start in different banks
 constexpr int kStageBytes = 16 * kStagePitch;
+constexpr int kStages = 3;
 
 template <typename T>
 struct Unpack;
@@ -108,41 +110,52 @@ struct Unpack<__nv_bfloat16> {
   }
 };
 
-template <typename S>
-H3_DEV float load_scale(const void* s, int64_t i) {
-  return to_f32(reinterpret_cast<const S*>(s)[i]);
+H3_DEV float load_scale(const Int4Args& a, int64_t i) {
+  if (a.scale_type == H3_TYPE_F32) return __ldg(reinterpret_cast<const float*>(a.scales) + i);
+  const uint16_t h = __ldg(reinterpret_cast<const uint16_t*>(a.scales) + i);
+  return a.scale_type == H3_TYPE_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
 }
 
-// A CTA: MT * 8 rows of x times 16 * WN columns, eight warps as WN column tiles by WK slices
-// of k (every WK-th stage), the slices added in order through shared memory at the end.
-// VEC: rows of packed weights start on 16-byte boundaries (k a multiple of 32), so they are
-// fetched by cp.async; else byte by byte.
-template <typename T, typename S, bool ZEROS, int MT, int WN, bool VEC, int STAGES>
-__global__ void __launch_bounds__(kInt4Warps * 32) int4_kernel(const __grid_constant__ Int4Args a) {
-  constexpr int WK = kInt4Warps / WN;
-  constexpr int kRows = 8 * MT;
+// A CTA takes MT * 8 rows of x and, in rounds, wn tiles of 16 columns; its 16 warps are wn
+// tiles by 16 / wn slices of k (every (16 / wn)-th stage), whose sums are added in order
+// through shared memory at the end of a round.  A warp's stages of all rounds are one
+// sequence, fetched kStages - 1 ahead.  Where x of all of k fits, it is staged once.
+// GB: 32-k blocks of a group.  VEC: rows of packed weights start on 16-byte boundaries (k a
+// multiple of 32), so they are fetched by cp.async; else byte by byte.
+template <typename T, bool ZEROS, int MT, int GB, bool VEC>
+__global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_constant__ Int4Args a) {
+  constexpr int kRows = 8 * MT, kThreads = kInt4Warps * 32;
+  constexpr int kGroups = kStageK / 32 / GB;  // groups of a stage
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  const int WN = a.wn, WK = kInt4Warps / WN;
   const int wn = warp % WN, wk = warp / WN;
-  uint8_t* const ring = smem + warp * STAGES * kStageBytes;
-  // x: kRows rows of `chunk` values, neighbouring rows half the banks apart, so that two
-  // rows' four 16-byte words of a k block fill all banks
-  const int x_pitch = a.chunk * 2 + 64;
-  uint8_t* const xs = smem + kInt4Warps * STAGES * kStageBytes;
-  const int n0 = (blockIdx.x * WN + wn) * 16;
   const int64_t m0 = (int64_t)blockIdx.y * kRows;
   const int rows = (int)min((int64_t)kRows, a.m - m0);
   const int stages = (a.k + kStageK - 1) / kStageK;
+  const int tiles = (a.n + 15) / 16, rounds = (tiles + WN * (int)gridDim.x - 1) / (WN * (int)gridDim.x);
+  uint8_t* const ring = smem + warp * kStages * kStageBytes;
+  // staged x: the rows that exist and one of zeros for those that do not; neighbouring rows
+  // half the banks apart, so that two rows' four 16-byte words of a k block fill all banks
+  const int x_pitch = a.chunk * 2 + 64;
+  uint8_t* const xs = smem + kInt4Warps * kStages * kStageBytes;
+  float* const sums = reinterpret_cast<float*>(xs + (rows + 1) * x_pitch);  // [wk][wn][row][16]
+  const uint8_t* x_row[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) x_row[j] = xs + min(j * 8 + g, rows) * x_pitch + t * 16;
 
-  // fetches this warp's stage `s` (its 16 columns, kStageK codes) into slot s / WK % STAGES
-  const auto fetch = [&](int s) {
-    if (s < stages && n0 < a.n) {
-      uint8_t* dst = ring + (s / WK) % STAGES * kStageBytes;
+  // the fetching side: stage f_stage of round f_round into slot f_slot
+  int f_round = 0, f_stage = wk, f_slot = 0;
+  const auto fetch = [&]() {
+    if (f_round < rounds && f_stage < stages) {
+      const int n0 = ((f_round * (int)gridDim.x + (int)blockIdx.x) * WN + wn) * 16;
+      uint8_t* dst = ring + f_slot * kStageBytes;
       if (VEC) {
+        const int byte = f_stage * (kStageK / 2) + (lane & 7) * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = i * 4 + (lane >> 3), byte = s * (kStageK / 2) + (lane & 7) * 16;
+          const int row = i * 4 + (lane >> 3);
           uint8_t* p = dst + row * kStagePitch + (lane & 7) * 16;
           if (n0 + row < a.n && byte < a.pitch)
             cp_async16((uint32_t)__cvta_generic_to_shared(p), a.w + (int64_t)(n0 + row) * a.pitch + byte);
@@ -150,150 +163,209 @@ __global__ void __launch_bounds__(kInt4Warps * 32) int4_kernel(const __grid_cons
         }
       } else {
         for (int i = lane; i < 16 * kStageK / 8; i += 32) {
-          const int row = i / (kStageK / 8), word = i % (kStageK / 8), byte = s * (kStageK / 2) + word * 4;
+          const int row = i / (kStageK / 8), word = i % (kStageK / 8), byte = f_stage * (kStageK / 2) + word * 4;
+          const uint8_t* src = a.w + (int64_t)(n0 + row) * a.pitch + byte;
           uint32_t v = 0;
-          for (int b = 0; b < 4; ++b)
-            if (n0 + row < a.n && byte + b < a.pitch)
-              v |= (uint32_t)a.w[(int64_t)(n0 + row) * a.pitch + byte + b] << (8 * b);
+          if (n0 + row < a.n) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (byte + b < a.pitch) v |= (uint32_t)__ldg(src + b) << (8 * b);
+          }
           *reinterpret_cast<uint32_t*>(dst + row * kStagePitch + word * 4) = v;
         }
       }
+      f_stage += WK;
+      if (f_stage >= stages) {
+        f_stage = wk;
+        ++f_round;
+      }
+      f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
     }
     cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) fetch(wk + i * WK);
+  for (int i = 0; i < kStages - 1; ++i) fetch();
 
-  float acc[MT][4];
-#pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-
-  const int col0 = min(n0 + g, a.n - 1), col1 = min(n0 + g + 8, a.n - 1);
-  const int64_t gi0 = (int64_t)col0 * a.groups, gi1 = (int64_t)col1 * a.groups;
-  int s = wk;  // this warp's next stage
-  for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
-    if (k0 > 0) __syncthreads();
-    // x of the chunk, zeros behind its rows and columns; the eight values of a word's codes
-    // in the order 0 4 1 5 2 6 3 7
+  // x of a chunk, zeros behind its columns; the eight values of a word's codes in the order
+  // 0 4 1 5 2 6 3 7
+  const auto stage_x = [&](int k0) {
     const int words = a.chunk / 8;
-    for (int i = threadIdx.x; i < kRows * words; i += kInt4Warps * 32) {
-      const int row = i / words, w = i - row * words, k = k0 + w * 8;
-      T v[8];
-      const T* src = reinterpret_cast<const T*>(a.x) + (m0 + row) * a.x_ld + k;
+    for (int row = warp; row <= rows; row += kInt4Warps) {
+      const T* src = reinterpret_cast<const T*>(a.x) + (m0 + row) * a.x_ld;
+      for (int w = lane; w < words; w += 32) {
+        const int k = k0 + w * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < rows && k < a.k) {
+          if (a.x_vec && k + 8 <= a.k) {
+            v = __ldg(reinterpret_cast<const uint4*>(src + k));
+          } else {
+            uint32_t h[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = row < rows && k + e < a.k ? src[e] : from_f32<T>(0.0f);
-      T o[8] = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
-      *reinterpret_cast<uint4*>(xs + row * x_pitch + w * 16) = *reinterpret_cast<uint4*>(o);
-    }
-    __syncthreads();
-    const int end = min(stages, (k0 + a.chunk) / kStageK);
-    for (; s < end; s += WK) {
-      cp_async_wait<STAGES - 2>();
-      __syncwarp();
-      const uint8_t* stage = ring + (s / WK) % STAGES * kStageBytes;
-      const uint8_t* xk = xs + (s * kStageK - k0) * 2 + t * 16;
-      const int blocks = min(kStageK, a.k - s * kStageK + 31) / 32;
-      int b = 0;
-      while (b < blocks) {
-        // one group: its scales and zeros, the products of its blocks, the scaled sum
-        const int gr = (s * (kStageK / 32) + b) >> a.group_shift;
-        const int stop = min(blocks, ((gr + 1) << a.group_shift) - s * (kStageK / 32));
-        const float s0 = load_scale<S>(a.scales, gi0 + gr), s1 = load_scale<S>(a.scales, gi1 + gr);
-        const Unpack<T> u0(ZEROS ? a.zeros[gi0 + gr] : 8), u1(ZEROS ? a.zeros[gi1 + gr] : 8);
-        float part[MT][4];
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part[j][i] = 0.0f;
-        for (; b < stop; ++b) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(stage + g * kStagePitch + b * 16 + t * 4);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(stage + (g + 8) * kStagePitch + b * 16 + t * 4);
-          uint32_t p0[4], p1[4];
-          u0(w0, p0);
-          u1(w1, p1);
-          const uint32_t first[4] = {p0[0], p1[0], p0[1], p1[1]}, second[4] = {p0[2], p1[2], p0[3], p1[3]};
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            const uint4 xv = *reinterpret_cast<const uint4*>(xk + (j * 8 + g) * x_pitch + b * 64);
-            Unpack<T>::mma(part[j], first, xv.x, xv.y);
-            Unpack<T>::mma(part[j], second, xv.z, xv.w);
+            for (int e = 0; e < 8; ++e)
+              if (k + e < a.k) h[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(src + k)[e] << (16 * (e & 1));
+            v = make_uint4(h[0], h[1], h[2], h[3]);
           }
         }
+        const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                                   __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        *reinterpret_cast<uint4*>(xs + row * x_pitch + w * 16) = o;
+      }
+    }
+  };
+
+  const bool once = a.chunk >= a.k;
+  int slot = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int n0 = ((round * (int)gridDim.x + (int)blockIdx.x) * WN + wn) * 16;
+    const int64_t at0 = (int64_t)min(n0 + g, a.n - 1) * a.groups, at1 = (int64_t)min(n0 + g + 8, a.n - 1) * a.groups;
+    float acc[MT][4];
 #pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          acc[j][0] = __fmaf_rn(s0, part[j][0], acc[j][0]);
-          acc[j][1] = __fmaf_rn(s0, part[j][1], acc[j][1]);
-          acc[j][2] = __fmaf_rn(s1, part[j][2], acc[j][2]);
-          acc[j][3] = __fmaf_rn(s1, part[j][3], acc[j][3]);
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+
+    int s = wk;
+    // scales and zeros of the group to come
+    float s0 = 0.0f, s1 = 0.0f;
+    int z0 = 8, z1 = 8;
+    const auto look = [&](int gr) {
+      if (gr < a.groups) {
+        s0 = load_scale(a, at0 + gr);
+        s1 = load_scale(a, at1 + gr);
+        if (ZEROS) {
+          z0 = __ldg(a.zeros + at0 + gr);
+          z1 = __ldg(a.zeros + at1 + gr);
         }
       }
-      __syncwarp();
-      fetch(s + (STAGES - 1) * WK);
+    };
+    look(s * kGroups);
+    for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
+      if (!once || round == 0) {
+        if (!once) __syncthreads();
+        stage_x(k0);
+        __syncthreads();
+      }
+      const int end = min(stages, (k0 + a.chunk) / kStageK);
+      for (; s < end; s += WK) {
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        const uint8_t* w_at = ring + slot * kStageBytes + g * kStagePitch + t * 4;
+        const int x_at = (s * kStageK - k0) * 2;
+#pragma unroll 1
+        for (int q = 0; q < kGroups; ++q) {
+          const int gr = s * kGroups + q;
+          if (gr >= a.groups) break;
+          const float f0 = s0, f1 = s1;
+          const Unpack<T> u0(z0), u1(z1);
+          look(q + 1 < kGroups ? gr + 1 : (s + WK) * kGroups);
+          float part[MT][4];
+#pragma unroll
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) part[j][i] = 0.0f;
+#pragma unroll
+          for (int b = 0; b < GB; ++b) {
+            const int block = q * GB + b;
+            uint32_t p0[4], p1[4];
+            u0(*reinterpret_cast<const uint32_t*>(w_at + block * 16), p0);
+            u1(*reinterpret_cast<const uint32_t*>(w_at + 8 * kStagePitch + block * 16), p1);
+            const uint32_t first[4] = {p0[0], p1[0], p0[1], p1[1]}, second[4] = {p0[2], p1[2], p0[3], p1[3]};
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              const uint4 xv = *reinterpret_cast<const uint4*>(x_row[j] + x_at + block * 64);
+              Unpack<T>::mma(part[j], first, xv.x, xv.y);
+              Unpack<T>::mma(part[j], second, xv.z, xv.w);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            acc[j][0] = __fmaf_rn(f0, part[j][0], acc[j][0]);
+            acc[j][1] = __fmaf_rn(f0, part[j][1], acc[j][1]);
+            acc[j][2] = __fmaf_rn(f1, part[j][2], acc[j][2]);
+            acc[j][3] = __fmaf_rn(f1, part[j][3], acc[j][3]);
+          }
+        }
+        __syncwarp();
+        fetch();  // into the slot of the stage before
+        slot = slot + 1 == kStages ? 0 : slot + 1;
+      }
     }
+
+    // the slices' sums through shared memory, added in order; then bias and store
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = j * 8 + 2 * t + (i & 1);
+        if (row < rows) sums[((wk * WN + wn) * rows + row) * 16 + g + (i >> 1) * 8] = acc[j][i];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < WN * rows * 16; i += kThreads) {
+      const int c = i % (16 * WN), row = i / (16 * WN);
+      const int n = (round * (int)gridDim.x + (int)blockIdx.x) * WN * 16 + c;
+      if (n >= a.n) continue;
+      float v = 0.0f;
+      for (int q = 0; q < WK; ++q) v += sums[((q * WN + c / 16) * rows + row) * 16 + c % 16];
+      if (a.bias != nullptr) v += __ldg(a.bias + n);
+      const int64_t at = (m0 + row) * a.n + n;
+      if (a.out_type == H3_TYPE_F32) reinterpret_cast<float*>(a.out)[at] = v;
+      else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
+    }
+    if (round + 1 < rounds) __syncthreads();
   }
   cp_async_wait<0>();
-
-  // the slices' sums through shared memory, added in order; then bias and store
-  __syncthreads();
-  float* sums = reinterpret_cast<float*>(smem);  // [WK][WN][kRows][16]
-#pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      sums[((wk * WN + wn) * kRows + j * 8 + 2 * t + (i & 1)) * 16 + g + (i >> 1) * 8] = acc[j][i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < WN * kRows * 16; i += kInt4Warps * 32) {
-    const int c = i % (16 * WN), row = i / (16 * WN), n = blockIdx.x * WN * 16 + c;
-    if (row >= rows || n >= a.n) continue;
-    float v = 0.0f;
-#pragma unroll
-    for (int q = 0; q < WK; ++q) v += sums[((q * WN + c / 16) * kRows + row) * 16 + c % 16];
-    if (a.bias != nullptr) v += __ldg(a.bias + n);
-    const int64_t at = (m0 + row) * a.n + n;
-    if (a.out_type == H3_TYPE_F32) reinterpret_cast<float*>(a.out)[at] = v;
-    else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
-  }
 }
 
-template <typename T, typename S, bool ZEROS, int MT, int WN, bool VEC>
-int launch_int4(Int4Args& a, cudaStream_t stream) {
-  constexpr int kStages = 4;
-  auto kern = int4_kernel<T, S, ZEROS, MT, WN, VEC, kStages>;
-  // x of all of k where it fits beside the weights' stages and a second CTA, else in chunks
-  const int ring = kInt4Warps * kStages * kStageBytes, budget = 110 * 1024 - ring;
-  const int all = (a.k + kStageK - 1) / kStageK * kStageK;
-  a.chunk = std::max(kStageK, std::min(all, (budget / (8 * MT) - 64) / 2 / kStageK * kStageK));
-  const int smem = std::max(ring + 8 * MT * (a.chunk * 2 + 64), (int)sizeof(float) * kInt4Warps * 8 * MT * 16);
+template <typename T, bool ZEROS, int MT, int GB, bool VEC>
+int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
+  auto kern = int4_kernel<T, ZEROS, MT, GB, VEC>;
+  // Column tiles at a time: the number that needs the fewest stages one after the other on
+  // the busiest SM; more slices of k (fewer tiles) where it makes no difference.
+  const int stages = (a.k + kStageK - 1) / kStageK, tiles = (a.n + 15) / 16;
+  const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
+  const int ctas = std::max(1, sms / blocks_m);
+  int64_t best = -1;
+  for (int wn = 1; wn <= kInt4Warps; wn *= 2) {
+    const int wk = kInt4Warps / wn;
+    const int64_t cost = (int64_t)((tiles + wn * ctas - 1) / (wn * ctas)) * ((stages + wk - 1) / wk);
+    if (best < 0 || cost < best) {
+      best = cost;
+      a.wn = wn;
+    }
+  }
+  // x of all of k where it fits beside the weights' stages and the sums, else in chunks
+  const int rows = (int)std::min<int64_t>(8 * MT, a.m);
+  const int fixed = kInt4Warps * (kStages * kStageBytes + rows * 16 * (int)sizeof(float));
+  const int all = stages * kStageK, room = (226 * 1024 - fixed) / (rows + 1) - 64;
+  a.chunk = std::min(all, room / 2 / kStageK * kStageK);
+  const int smem = fixed + (rows + 1) * (a.chunk * 2 + 64);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return H3_ERR_CUDA;
   }
-  const dim3 grid((a.n + 16 * WN - 1) / (16 * WN), (unsigned)((a.m + 8 * MT - 1) / (8 * MT)));
+  const dim3 grid(std::min(ctas, (tiles + a.wn - 1) / a.wn), blocks_m);
   kern<<<grid, kInt4Warps * 32, smem, stream>>>(a);
   return h3host::check_launch();
 }
 
-template <typename T, typename S, bool ZEROS>
+template <typename T, bool ZEROS, int GB>
 int launch_int4_shape(Int4Args& a, int sms, cudaStream_t stream) {
-  const bool vec = a.k % 32 == 0 && h3host::aligned(a.w, 16);
-  if (!vec) return a.m <= 8 ? launch_int4<T, S, ZEROS, 1, 2, false>(a, stream)
-                            : launch_int4<T, S, ZEROS, 4, 2, false>(a, stream);
-  if (a.m <= 8) return launch_int4<T, S, ZEROS, 1, 2, true>(a, stream);
-  if (a.m <= 16) return launch_int4<T, S, ZEROS, 2, 2, true>(a, stream);
-  return launch_int4<T, S, ZEROS, 4, 2, true>(a, stream);
+  if (a.k % 32 != 0 || !h3host::aligned(a.w, 16))
+    return a.m <= 8 ? launch_int4<T, ZEROS, 1, GB, false>(a, sms, stream)
+                    : launch_int4<T, ZEROS, 4, GB, false>(a, sms, stream);
+  if (a.m <= 8) return launch_int4<T, ZEROS, 1, GB, true>(a, sms, stream);
+  if (a.m <= 16) return launch_int4<T, ZEROS, 2, GB, true>(a, sms, stream);
+  return launch_int4<T, ZEROS, 4, GB, true>(a, sms, stream);
 }
 
 template <typename T>
-int launch_int4_type(Int4Args& a, int scale_type, int sms, cudaStream_t stream) {
+int launch_int4_type(Int4Args& a, int group, int sms, cudaStream_t stream) {
   const bool z = a.zeros != nullptr;
-  if (scale_type == H3_TYPE_F32)
-    return z ? launch_int4_shape<T, float, true>(a, sms, stream) : launch_int4_shape<T, float, false>(a, sms, stream);
-  if (scale_type == H3_TYPE_F16)
-    return z ? launch_int4_shape<T, __half, true>(a, sms, stream) : launch_int4_shape<T, __half, false>(a, sms, stream);
-  return z ? launch_int4_shape<T, __nv_bfloat16, true>(a, sms, stream)
-           : launch_int4_shape<T, __nv_bfloat16, false>(a, sms, stream);
+  if (group == 32)
+    return z ? launch_int4_shape<T, true, 1>(a, sms, stream) : launch_int4_shape<T, false, 1>(a, sms, stream);
+  if (group == 64)
+    return z ? launch_int4_shape<T, true, 2>(a, sms, stream) : launch_int4_shape<T, false, 2>(a, sms, stream);
+  return z ? launch_int4_shape<T, true, 4>(a, sms, stream) : launch_int4_shape<T, false, 4>(a, sms, stream);
 }
 
 }  // namespace h3
@@ -317,9 +389,10 @@ extern "C" int h3_int4_linear(const void* x, int x_type, int64_t x_ld, int64_t m
   h3host::DeviceScope scope;
   if (int s = scope.bind(x, &dev)) return s;
   Int4Args a{x, x_ld, m, (int)k, (int)n, w, scales, zeros, bias, out, (int)((k + group - 1) / group),
-             (int)((k + 1) / 2), group == 32 ? 0 : group == 64 ? 1 : 2, 0, out_type};
+             (int)((k + 1) / 2), scale_type, out_type, 0, 0,
+             h3host::aligned(x, 16) && (m == 1 || x_ld % 8 == 0)};
   cudaStream_t st = (cudaStream_t)stream;
   const int sms = h3host::sm_count(dev);
-  return x_type == H3_TYPE_F16 ? launch_int4_type<__half>(a, scale_type, sms, st)
-                               : launch_int4_type<__nv_bfloat16>(a, scale_type, sms, st);
+  return x_type == H3_TYPE_F16 ? launch_int4_type<__half>(a, group, sms, st)
+                               : launch_int4_type<__nv_bfloat16>(a, group, sms, st);
 }
