@@ -54,12 +54,8 @@ template <>
 struct Unpack<__half> {
   uint32_t low, high;  // -(1024 + zero) and -(64 + zero) in both halves
 
-  H3_DEV explicit Unpack(int zero) {
-    const __half2 a = __half2half2(__float2half_rn(-(1024.0f + (float)zero)));
-    const __half2 b = __half2half2(__float2half_rn(-(64.0f + (float)zero)));
-    low = *reinterpret_cast<const uint32_t*>(&a);
-    high = *reinterpret_cast<const uint32_t*>(&b);
-  }
+  // the bits of -1024 and -64, and what one more adds to them
+  H3_DEV explicit Unpack(uint32_t zero) : low(0xe400e400u + zero * 0x00010001u), high(0xd400d400u + zero * 0x00100010u) {}
   H3_DEV void operator()(uint32_t w, uint32_t (&p)[4]) const {
     const uint32_t v = w >> 8;
     p[0] = add((w & 0x000f000fu) | 0x64006400u, low);
@@ -84,16 +80,20 @@ struct Unpack<__half> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  H3_DEV static void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // onto zeros
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  }
 };
 
 template <>
 struct Unpack<__nv_bfloat16> {
   uint32_t low;  // -(128 + zero) in both halves
 
-  H3_DEV explicit Unpack(int zero) {
-    const __nv_bfloat162 a = __bfloat162bfloat162(__float2bfloat16_rn(-(128.0f + (float)zero)));
-    low = *reinterpret_cast<const uint32_t*>(&a);
-  }
+  H3_DEV explicit Unpack(uint32_t zero) : low(0xc300c300u + zero * 0x00010001u) {}
   H3_DEV void operator()(uint32_t w, uint32_t (&p)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -108,12 +108,25 @@ struct Unpack<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  H3_DEV static void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // onto zeros
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  }
 };
 
-H3_DEV float load_scale(const Int4Args& a, int64_t i) {
-  if (a.scale_type == H3_TYPE_F32) return __ldg(reinterpret_cast<const float*>(a.scales) + i);
-  const uint16_t h = __ldg(reinterpret_cast<const uint16_t*>(a.scales) + i);
-  return a.scale_type == H3_TYPE_F16 ? __half2float(__ushort_as_half(h)) : __uint_as_float((uint32_t)h << 16);
+// A scale as it lies in memory (S: 4 bytes, fp32, or 2, fp16 or bf16), to fp32.
+H3_DEV float scale_value(uint32_t bits, int) { return __uint_as_float(bits); }
+H3_DEV float scale_value(uint16_t bits, int type) {
+  return type == H3_TYPE_F16 ? __half2float(__ushort_as_half(bits)) : __uint_as_float((uint32_t)bits << 16);
+}
+
+// Barrier of the `warps` warps that share a column tile (id 1 and up: 0 is the CTA's).
+H3_DEV void tile_barrier(int id, int warps) {
+  if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(warps * 32) : "memory");
+  else __syncwarp();
 }
 
 // A CTA takes MT * 8 rows of x and, in rounds, wn tiles of 16 columns; its 16 warps are wn
@@ -122,9 +135,9 @@ H3_DEV float load_scale(const Int4Args& a, int64_t i) {
 // sequence, fetched kStages - 1 ahead.  Where x of all of k fits, it is staged once.
 // GB: 32-k blocks of a group.  VEC: rows of packed weights start on 16-byte boundaries (k a
 // multiple of 32), so they are fetched by cp.async; else byte by byte.
-template <typename T, bool ZEROS, int MT, int GB, bool VEC>
+template <typename T, typename S, bool ZEROS, int MT, int GB, bool VEC>
 __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_constant__ Int4Args a) {
-  constexpr int kRows = 8 * MT, kThreads = kInt4Warps * 32;
+  constexpr int kRows = 8 * MT;
   constexpr int kGroups = kStageK / 32 / GB;  // groups of a stage
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,7 +153,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   // half the banks apart, so that two rows' four 16-byte words of a k block fill all banks
   const int x_pitch = a.chunk * 2 + 64;
   uint8_t* const xs = smem + kInt4Warps * kStages * kStageBytes;
-  float* const sums = reinterpret_cast<float*>(xs + (rows + 1) * x_pitch);  // [wk][wn][row][16]
+  float* const sums = reinterpret_cast<float*>(xs + (rows + 1) * x_pitch);  // [wn][wk][row][16]
   const uint8_t* x_row[MT];
 #pragma unroll
   for (int j = 0; j < MT; ++j) x_row[j] = xs + min(j * 8 + g, rows) * x_pitch + t * 16;
@@ -225,20 +238,26 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
 
     int s = wk;
-    // scales and zeros of the group to come
-    float s0 = 0.0f, s1 = 0.0f;
-    int z0 = 8, z1 = 8;
-    const auto look = [&](int gr) {
-      if (gr < a.groups) {
-        s0 = load_scale(a, at0 + gr);
-        s1 = load_scale(a, at1 + gr);
+    // scales and zeros of the stage to come; a scale of 0 behind the last group
+    S scale[kGroups][2];
+    uint8_t zero[kGroups][2];
+    const auto look = [&](int stage) {
+      const S* p0 = reinterpret_cast<const S*>(a.scales) + at0 + stage * kGroups;
+      const S* p1 = reinterpret_cast<const S*>(a.scales) + at1 + stage * kGroups;
+      const uint8_t* z0 = a.zeros + at0 + stage * kGroups;
+      const uint8_t* z1 = a.zeros + at1 + stage * kGroups;
+      const int left = a.groups - stage * kGroups;
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        scale[q][0] = q < left ? __ldg(p0 + q) : (S)0;
+        scale[q][1] = q < left ? __ldg(p1 + q) : (S)0;
         if (ZEROS) {
-          z0 = __ldg(a.zeros + at0 + gr);
-          z1 = __ldg(a.zeros + at1 + gr);
+          zero[q][0] = q < left ? __ldg(z0 + q) : (uint8_t)0;
+          zero[q][1] = q < left ? __ldg(z1 + q) : (uint8_t)0;
         }
       }
     };
-    look(s * kGroups);
+    look(s);
     for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
       if (!once || round == 0) {
         if (!once) __syncthreads();
@@ -247,22 +266,24 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
       }
       const int end = min(stages, (k0 + a.chunk) / kStageK);
       for (; s < end; s += WK) {
+        S now[kGroups][2];
+        uint32_t offset[kGroups][2];
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            now[q][i] = scale[q][i];
+            offset[q][i] = ZEROS ? zero[q][i] : 8;
+          }
+        look(s + WK);
         cp_async_wait<kStages - 2>();
         __syncwarp();
         const uint8_t* w_at = ring + slot * kStageBytes + g * kStagePitch + t * 4;
         const int x_at = (s * kStageK - k0) * 2;
-#pragma unroll 1
+#pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-          const int gr = s * kGroups + q;
-          if (gr >= a.groups) break;
-          const float f0 = s0, f1 = s1;
-          const Unpack<T> u0(z0), u1(z1);
-          look(q + 1 < kGroups ? gr + 1 : (s + WK) * kGroups);
+          const Unpack<T> u0(offset[q][0]), u1(offset[q][1]);
           float part[MT][4];
-#pragma unroll
-          for (int j = 0; j < MT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part[j][i] = 0.0f;
 #pragma unroll
           for (int b = 0; b < GB; ++b) {
             const int block = q * GB + b;
@@ -273,10 +294,12 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
               const uint4 xv = *reinterpret_cast<const uint4*>(x_row[j] + x_at + block * 64);
-              Unpack<T>::mma(part[j], first, xv.x, xv.y);
+              if (b == 0) Unpack<T>::mma0(part[j], first, xv.x, xv.y);
+              else Unpack<T>::mma(part[j], first, xv.x, xv.y);
               Unpack<T>::mma(part[j], second, xv.z, xv.w);
             }
           }
+          const float f0 = scale_value(now[q][0], a.scale_type), f1 = scale_value(now[q][1], a.scale_type);
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
             acc[j][0] = __fmaf_rn(f0, part[j][0], acc[j][0]);
@@ -291,43 +314,46 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
       }
     }
 
-    // the slices' sums through shared memory, added in order; then bias and store
+    // the slices' sums through shared memory, added in order; then bias and store.  Only the
+    // warps of one tile wait for one another.
+    float* const tile = sums + wn * WK * rows * 16;
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = j * 8 + 2 * t + (i & 1);
-        if (row < rows) sums[((wk * WN + wn) * rows + row) * 16 + g + (i >> 1) * 8] = acc[j][i];
+        if (row < rows) tile[(wk * rows + row) * 16 + g + (i >> 1) * 8] = acc[j][i];
       }
-    __syncthreads();
-    for (int i = threadIdx.x; i < WN * rows * 16; i += kThreads) {
-      const int c = i % (16 * WN), row = i / (16 * WN);
-      const int n = (round * (int)gridDim.x + (int)blockIdx.x) * WN * 16 + c;
+    tile_barrier(1 + wn, WK);
+    for (int i = wk * 32 + lane; i < rows * 16; i += WK * 32) {
+      const int n = n0 + (i & 15), row = i >> 4;
       if (n >= a.n) continue;
       float v = 0.0f;
-      for (int q = 0; q < WK; ++q) v += sums[((q * WN + c / 16) * rows + row) * 16 + c % 16];
+      for (int q = 0; q < WK; ++q) v += tile[q * rows * 16 + i];
       if (a.bias != nullptr) v += __ldg(a.bias + n);
       const int64_t at = (m0 + row) * a.n + n;
       if (a.out_type == H3_TYPE_F32) reinterpret_cast<float*>(a.out)[at] = v;
       else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
     }
-    if (round + 1 < rounds) __syncthreads();
+    tile_barrier(1 + wn, WK);
   }
   cp_async_wait<0>();
 }
 
-template <typename T, bool ZEROS, int MT, int GB, bool VEC>
+template <typename T, typename S, bool ZEROS, int MT, int GB, bool VEC>
 int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
-  auto kern = int4_kernel<T, ZEROS, MT, GB, VEC>;
+  auto kern = int4_kernel<T, S, ZEROS, MT, GB, VEC>;
   // Column tiles at a time: the number that needs the fewest stages one after the other on
-  // the busiest SM; more slices of k (fewer tiles) where it makes no difference.
+  // the busiest SM.
   const int stages = (a.k + kStageK - 1) / kStageK, tiles = (a.n + 15) / 16;
   const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
   const int ctas = std::max(1, sms / blocks_m);
   int64_t best = -1;
   for (int wn = 1; wn <= kInt4Warps; wn *= 2) {
     const int wk = kInt4Warps / wn;
-    const int64_t cost = (int64_t)((tiles + wn * ctas - 1) / (wn * ctas)) * ((stages + wk - 1) / wk);
+    // in quarters of a stage; joining slices costs about as much as one stage
+    const int64_t cost = (int64_t)((tiles + wn * ctas - 1) / (wn * ctas)) *
+                         (4 * ((stages + wk - 1) / wk) + (wk > 1 ? 4 : 1));
     if (best < 0 || cost < best) {
       best = cost;
       a.wn = wn;
@@ -348,24 +374,31 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   return h3host::check_launch();
 }
 
-template <typename T, bool ZEROS, int GB>
+template <typename T, typename S, bool ZEROS, int GB>
 int launch_int4_shape(Int4Args& a, int sms, cudaStream_t stream) {
   if (a.k % 32 != 0 || !h3host::aligned(a.w, 16))
-    return a.m <= 8 ? launch_int4<T, ZEROS, 1, GB, false>(a, sms, stream)
-                    : launch_int4<T, ZEROS, 4, GB, false>(a, sms, stream);
-  if (a.m <= 8) return launch_int4<T, ZEROS, 1, GB, true>(a, sms, stream);
-  if (a.m <= 16) return launch_int4<T, ZEROS, 2, GB, true>(a, sms, stream);
-  return launch_int4<T, ZEROS, 4, GB, true>(a, sms, stream);
+    return a.m <= 8 ? launch_int4<T, S, ZEROS, 1, GB, false>(a, sms, stream)
+                    : launch_int4<T, S, ZEROS, 4, GB, false>(a, sms, stream);
+  if (a.m <= 8) return launch_int4<T, S, ZEROS, 1, GB, true>(a, sms, stream);
+  if (a.m <= 16) return launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream);
+  return launch_int4<T, S, ZEROS, 4, GB, true>(a, sms, stream);
+}
+
+template <typename T, typename S, bool ZEROS>
+int launch_int4_group(Int4Args& a, int group, int sms, cudaStream_t stream) {
+  if (group == 32) return launch_int4_shape<T, S, ZEROS, 1>(a, sms, stream);
+  if (group == 64) return launch_int4_shape<T, S, ZEROS, 2>(a, sms, stream);
+  return launch_int4_shape<T, S, ZEROS, 4>(a, sms, stream);
 }
 
 template <typename T>
 int launch_int4_type(Int4Args& a, int group, int sms, cudaStream_t stream) {
   const bool z = a.zeros != nullptr;
-  if (group == 32)
-    return z ? launch_int4_shape<T, true, 1>(a, sms, stream) : launch_int4_shape<T, false, 1>(a, sms, stream);
-  if (group == 64)
-    return z ? launch_int4_shape<T, true, 2>(a, sms, stream) : launch_int4_shape<T, false, 2>(a, sms, stream);
-  return z ? launch_int4_shape<T, true, 4>(a, sms, stream) : launch_int4_shape<T, false, 4>(a, sms, stream);
+  if (a.scale_type == H3_TYPE_F32)
+    return z ? launch_int4_group<T, uint32_t, true>(a, group, sms, stream)
+             : launch_int4_group<T, uint32_t, false>(a, group, sms, stream);
+  return z ? launch_int4_group<T, uint16_t, true>(a, group, sms, stream)
+           : launch_int4_group<T, uint16_t, false>(a, group, sms, stream);
 }
 
 }  // namespace h3
