@@ -12,10 +12,13 @@
 // weights in shared memory, four times the bytes of the packed ones; at so few rows the
 // older instruction is far from its limit.)
 //
-// The order of k inside a product does not matter as long as both operands agree, so the
-// weights need no layout of their own: in a block of 32 k, lane t of a row's four takes the
-// 4-byte word t of the packed row, codes 8 t to 8 t + 7, and the x staged in shared memory
-// is permuted to match the pairs that the unpacking yields, (0, 4), (1, 5), (2, 6), (3, 7).
+// The order of k inside a product does not matter as long as both operands agree and a
+// product stays inside a group, so the weights need no layout of their own: lane t of a row's
+// four takes the t-th quarter of each group's bytes in one read of 4, 8 or 16 bytes, and x,
+// staged in shared memory, is permuted to match the pairs that the unpacking of a 4-byte word
+// yields, (0, 4), (1, 5), (2, 6), (3, 7).  Weights come through cp.async, two stages ahead;
+// straight into registers they left too few bytes in flight (44 against 33 us at 9 x 5376 x
+// 32256).
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -37,11 +40,17 @@ struct Int4Args {
 };
 
 constexpr int kInt4Warps = 16;
-constexpr int kStageK = 256;                   // k of one stage of packed weights
-constexpr int kStagePitch = kStageK / 2 + 16;  // bytes of a stage's row: the eight rows that a
-                                               // load touches start in different banks
-constexpr int kStageBytes = 16 * kStagePitch;
+constexpr int kStageK = 256;  // k of one stage of a warp
 constexpr int kStages = 3;
+constexpr int kStageBytes = 16 * kStageK / 2;
+
+// (a & MASK) | b in one instruction, which takes one constant and not two.
+template <uint32_t MASK>
+H3_DEV uint32_t masked_onto(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "n"(MASK), "r"(b));
+  return r;
+}
 
 template <typename T>
 struct Unpack;
@@ -58,10 +67,10 @@ struct Unpack<__half> {
   H3_DEV explicit Unpack(uint32_t zero) : low(0xe400e400u + zero * 0x00010001u), high(0xd400d400u + zero * 0x00100010u) {}
   H3_DEV void operator()(uint32_t w, uint32_t (&p)[4]) const {
     const uint32_t v = w >> 8;
-    p[0] = add((w & 0x000f000fu) | 0x64006400u, low);
-    p[1] = fma((w & 0x00f000f0u) | 0x64006400u, high);
-    p[2] = add((v & 0x000f000fu) | 0x64006400u, low);
-    p[3] = fma((v & 0x00f000f0u) | 0x64006400u, high);
+    p[0] = add(masked_onto<0x000f000fu>(w, 0x64006400u), low);
+    p[1] = fma(masked_onto<0x00f000f0u>(w, 0x64006400u), high);
+    p[2] = add(masked_onto<0x000f000fu>(v, 0x64006400u), low);
+    p[3] = fma(masked_onto<0x00f000f0u>(v, 0x64006400u), high);
   }
   H3_DEV static uint32_t add(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -99,7 +108,7 @@ struct Unpack<__nv_bfloat16> {
     for (int i = 0; i < 4; ++i)
       asm("fma.rn.bf16x2 %0, %1, %2, %3;"
           : "=r"(p[i])
-          : "r"(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u), "r"(0x3f803f80u), "r"(low));
+          : "r"(masked_onto<0x000f000fu>(w >> (4 * i), 0x43004300u)), "r"(0x3f803f80u), "r"(low));
   }
   H3_DEV static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -148,65 +157,86 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   const int rows = (int)min((int64_t)kRows, a.m - m0);
   const int stages = (a.k + kStageK - 1) / kStageK;
   const int tiles = (a.n + 15) / 16, rounds = (tiles + WN * (int)gridDim.x - 1) / (WN * (int)gridDim.x);
-  uint8_t* const ring = smem + warp * kStages * kStageBytes;
-  // staged x: the rows that exist and one of zeros for those that do not; neighbouring rows
-  // half the banks apart, so that two rows' four 16-byte words of a k block fill all banks
+  // staged x: the rows that exist and one of zeros for those that do not, in 16-byte units of
+  // the eight values of a word's codes.  At one step the lanes of a row read every GB-th unit,
+  // so the units of four neighbours are exchanged by the number of their four, and
+  // neighbouring rows lie half the banks apart: no two of eight lanes meet in a bank.
   const int x_pitch = a.chunk * 2 + 64;
+  uint8_t* const ring = smem + warp * kStages * kStageBytes;
   uint8_t* const xs = smem + kInt4Warps * kStages * kStageBytes;
   float* const sums = reinterpret_cast<float*>(xs + (rows + 1) * x_pitch);  // [wn][wk][row][16]
   const uint8_t* x_row[MT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) x_row[j] = xs + min(j * 8 + g, rows) * x_pitch + t * 16;
+  for (int j = 0; j < MT; ++j) x_row[j] = xs + min(j * 8 + g, rows) * x_pitch;
+  int x_unit[4];  // of this lane at step i of 128 k
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int u = GB == 4 ? 4 * t + i : GB == 2 ? 8 * (i >> 1) + 2 * t + (i & 1) : 4 * i + t;
+    x_unit[i] = ((u & ~3) | ((u ^ (u >> 2)) & 3)) * 16;
+  }
 
-  // the fetching side: stage f_stage of round f_round into slot f_slot
+  // A stage in its slot: 16 rows of 128 bytes, the 16-byte words of a row exchanged so that
+  // the rows that one read of a quarter touches at once fill all banks.
+  const auto exchanged = [](int row) { return GB == 4 ? (row & 1) << 2 : GB == 2 ? (row & 3) << 1 : row & 7; };
+  const int w_unit = GB == 4 ? t : GB == 2 ? t >> 1 : 0, w_byte = GB == 4 ? 0 : GB == 2 ? (t & 1) * 8 : t * 4;
+
+  // the fetching side: stages wk, wk + WK, ... of this warp's tile of every round; rows
+  // behind the last column are read as the last.  Behind a row's end a slot keeps any codes:
+  // x is 0 there, and so are the scales.
   int f_round = 0, f_stage = wk, f_slot = 0;
+  const uint8_t* f_src = nullptr;
+  const auto f_open = [&]() {
+    const int n0 = ((f_round * (int)gridDim.x + (int)blockIdx.x) * WN + wn) * 16;
+    f_src = a.w + (int64_t)min(n0, a.n - 1) * a.pitch;
+  };
   const auto fetch = [&]() {
     if (f_round < rounds && f_stage < stages) {
       const int n0 = ((f_round * (int)gridDim.x + (int)blockIdx.x) * WN + wn) * 16;
+      const int last = max(min(15, a.n - 1 - n0), 0);  // row of the tile
       uint8_t* dst = ring + f_slot * kStageBytes;
       if (VEC) {
         const int byte = f_stage * (kStageK / 2) + (lane & 7) * 16;
+        if (byte < a.pitch) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = i * 4 + (lane >> 3);
-          uint8_t* p = dst + row * kStagePitch + (lane & 7) * 16;
-          if (n0 + row < a.n && byte < a.pitch)
-            cp_async16((uint32_t)__cvta_generic_to_shared(p), a.w + (int64_t)(n0 + row) * a.pitch + byte);
-          else *reinterpret_cast<uint4*>(p) = make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 4 + (lane >> 3);
+            cp_async16((uint32_t)__cvta_generic_to_shared(dst + row * 128 + (((lane & 7) ^ exchanged(row)) << 4)),
+                       f_src + (int64_t)min(row, last) * a.pitch + byte);
+          }
         }
       } else {
         for (int i = lane; i < 16 * kStageK / 8; i += 32) {
           const int row = i / (kStageK / 8), word = i % (kStageK / 8), byte = f_stage * (kStageK / 2) + word * 4;
-          const uint8_t* src = a.w + (int64_t)(n0 + row) * a.pitch + byte;
+          const uint8_t* src = f_src + (int64_t)min(row, last) * a.pitch + byte;
           uint32_t v = 0;
-          if (n0 + row < a.n) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (byte + b < a.pitch) v |= (uint32_t)__ldg(src + b) << (8 * b);
-          }
-          *reinterpret_cast<uint32_t*>(dst + row * kStagePitch + word * 4) = v;
+          for (int b = 0; b < 4; ++b)
+            if (byte + b < a.pitch) v |= (uint32_t)__ldg(src + b) << (8 * b);
+          *reinterpret_cast<uint32_t*>(dst + row * 128 + (((word >> 2) ^ exchanged(row)) << 4) + (word & 3) * 4) = v;
         }
       }
       f_stage += WK;
       if (f_stage >= stages) {
         f_stage = wk;
         ++f_round;
+        f_open();
       }
       f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
     }
     cp_async_commit();
   };
+  f_open();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
-  // x of a chunk, zeros behind its columns; the eight values of a word's codes in the order
-  // 0 4 1 5 2 6 3 7
+  // x of a chunk, zeros behind its columns; a unit's eight values in the order 0 4 1 5 2 6 3 7
   const auto stage_x = [&](int k0) {
-    const int words = a.chunk / 8;
-    for (int row = warp; row <= rows; row += kInt4Warps) {
-      const T* src = reinterpret_cast<const T*>(a.x) + (m0 + row) * a.x_ld;
-      for (int w = lane; w < words; w += 32) {
-        const int k = k0 + w * 8;
+    const int units = a.chunk / 8, total = (rows + 1) * units;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < total; i += kInt4Warps * 32) {
+      {
+        const int row = i / units, u = i - row * units, k = k0 + u * 8;
+        const T* src = reinterpret_cast<const T*>(a.x) + (m0 + row) * a.x_ld;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (row < rows && k < a.k) {
           if (a.x_vec && k + 8 <= a.k) {
@@ -221,7 +251,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
         }
         const uint4 o = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                                    __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        *reinterpret_cast<uint4*>(xs + row * x_pitch + w * 16) = o;
+        *reinterpret_cast<uint4*>(xs + row * x_pitch + ((u & ~3) | ((u ^ (u >> 2)) & 3)) * 16) = o;
       }
     }
   };
@@ -230,33 +260,27 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   int slot = 0;
   for (int round = 0; round < rounds; ++round) {
     const int n0 = ((round * (int)gridDim.x + (int)blockIdx.x) * WN + wn) * 16;
-    const int64_t at0 = (int64_t)min(n0 + g, a.n - 1) * a.groups, at1 = (int64_t)min(n0 + g + 8, a.n - 1) * a.groups;
     float acc[MT][4];
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
 
-    int s = wk;
     // scales and zeros of the stage to come; a scale of 0 behind the last group
-    S scale[kGroups][2];
-    uint8_t zero[kGroups][2];
+    S scale[2][kGroups];
+    uint8_t zero[2][kGroups];
+    const int64_t group0[2] = {(int64_t)min(n0 + g, a.n - 1) * a.groups, (int64_t)min(n0 + g + 8, a.n - 1) * a.groups};
     const auto look = [&](int stage) {
-      const S* p0 = reinterpret_cast<const S*>(a.scales) + at0 + stage * kGroups;
-      const S* p1 = reinterpret_cast<const S*>(a.scales) + at1 + stage * kGroups;
-      const uint8_t* z0 = a.zeros + at0 + stage * kGroups;
-      const uint8_t* z1 = a.zeros + at1 + stage * kGroups;
-      const int left = a.groups - stage * kGroups;
+      const int first = stage * kGroups, left = a.groups - first;
 #pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        scale[q][0] = q < left ? __ldg(p0 + q) : (S)0;
-        scale[q][1] = q < left ? __ldg(p1 + q) : (S)0;
-        if (ZEROS) {
-          zero[q][0] = q < left ? __ldg(z0 + q) : (uint8_t)0;
-          zero[q][1] = q < left ? __ldg(z1 + q) : (uint8_t)0;
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+          scale[r][q] = q < left ? __ldg(reinterpret_cast<const S*>(a.scales) + group0[r] + first + q) : (S)0;
+          if (ZEROS) zero[r][q] = q < left ? __ldg(a.zeros + group0[r] + first + q) : (uint8_t)0;
         }
-      }
     };
+    int s = wk;
     look(s);
     for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
       if (!once || round == 0) {
@@ -265,41 +289,58 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
         __syncthreads();
       }
       const int end = min(stages, (k0 + a.chunk) / kStageK);
+#pragma unroll 1
       for (; s < end; s += WK) {
-        S now[kGroups][2];
-        uint32_t offset[kGroups][2];
+        S now[2][kGroups];
+        uint32_t offset[2][kGroups];
 #pragma unroll
-        for (int q = 0; q < kGroups; ++q)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            now[q][i] = scale[q][i];
-            offset[q][i] = ZEROS ? zero[q][i] : 8;
+          for (int q = 0; q < kGroups; ++q) {
+            now[r][q] = scale[r][q];
+            offset[r][q] = ZEROS ? zero[r][q] : 8;
           }
         look(s + WK);
         cp_async_wait<kStages - 2>();
         __syncwarp();
-        const uint8_t* w_at = ring + slot * kStageBytes + g * kStagePitch + t * 4;
+        const uint8_t* w_row = ring + slot * kStageBytes + g * 128 + w_byte;
         const int x_at = (s * kStageK - k0) * 2;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-          const Unpack<T> u0(offset[q][0]), u1(offset[q][1]);
+          uint32_t w[2][GB];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            // rows g and g + 8 are exchanged alike
+            const uint8_t* p = w_row + r * 1024 + (((q * GB + w_unit) ^ exchanged(g)) << 4);
+            if (GB == 4) {
+              const uint4 v = *reinterpret_cast<const uint4*>(p);
+              w[r][0] = v.x; w[r][1 % GB] = v.y; w[r][2 % GB] = v.z; w[r][3 % GB] = v.w;
+            } else if (GB == 2) {
+              const uint2 v = *reinterpret_cast<const uint2*>(p);
+              w[r][0] = v.x; w[r][1 % GB] = v.y;
+            } else {
+              w[r][0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+          }
+          const Unpack<T> u0(offset[0][q]), u1(offset[1][q]);
           float part[MT][4];
 #pragma unroll
-          for (int b = 0; b < GB; ++b) {
-            const int block = q * GB + b;
+          for (int i = 0; i < GB; ++i) {
+            const int block = q * GB + i;
             uint32_t p0[4], p1[4];
-            u0(*reinterpret_cast<const uint32_t*>(w_at + block * 16), p0);
-            u1(*reinterpret_cast<const uint32_t*>(w_at + 8 * kStagePitch + block * 16), p1);
+            u0(w[0][i], p0);
+            u1(w[1][i], p1);
             const uint32_t first[4] = {p0[0], p1[0], p0[1], p1[1]}, second[4] = {p0[2], p1[2], p0[3], p1[3]};
 #pragma unroll
             for (int j = 0; j < MT; ++j) {
-              const uint4 xv = *reinterpret_cast<const uint4*>(x_row[j] + x_at + block * 64);
-              if (b == 0) Unpack<T>::mma0(part[j], first, xv.x, xv.y);
+              const uint4 xv =
+                  *reinterpret_cast<const uint4*>(x_row[j] + x_at + x_unit[block & 3] + (block >> 2) * 256);
+              if (i == 0) Unpack<T>::mma0(part[j], first, xv.x, xv.y);
               else Unpack<T>::mma(part[j], first, xv.x, xv.y);
               Unpack<T>::mma(part[j], second, xv.z, xv.w);
             }
           }
-          const float f0 = scale_value(now[q][0], a.scale_type), f1 = scale_value(now[q][1], a.scale_type);
+          const float f0 = scale_value(now[0][q], a.scale_type), f1 = scale_value(now[1][q], a.scale_type);
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
             acc[j][0] = __fmaf_rn(f0, part[j][0], acc[j][0]);
