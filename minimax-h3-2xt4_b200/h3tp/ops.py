@@ -51,7 +51,7 @@ def _vec(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     t = _need(t, torch.float32, name)
     if t.numel() != n:
         raise ValueError(f"{name}: {n} values required, got {t.numel()}")
-    return t.reshape(-1)
+    return t if t.ndim == 1 else t.reshape(-1)
 
 
 INPUT_KINDS = {"gateup_f16": N.IN_GATEUP_F16, "act_f32": N.IN_ACT_F32, "act_f16": N.IN_ACT_F16}
@@ -493,10 +493,16 @@ _NORM_KINDS = {"rms": N.NORM_RMS, "layer": N.NORM_LAYER}
 _POSITIONS = {torch.int32: N.POS_I32, torch.int64: N.POS_I64, torch.float32: N.POS_F32}
 
 
-def _inference(where: str, device, **tensors) -> None:
+def _raw_stream(device: torch.device) -> int:
+    """The handle of the device's current stream (without a Stream object: a call on one row
+    or token is bound by its host side)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _inference(where: str, device, tensors, names) -> None:
     """Every tensor on `device`, none that autograd would have to follow."""
     grad = torch.is_grad_enabled()
-    for name, t in tensors.items():
+    for t, name in zip(tensors, names):
         if t is None:
             continue
         if t.device != device:
@@ -510,13 +516,22 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     """The addresses [first, last) that a strided tensor's elements lie in."""
     if t.numel() == 0:
         return 0, 0
-    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if t.is_contiguous():
+        last = t.numel()
+    else:
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + last * t.element_size()
 
 
 def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     (a0, a1), (b0, b1) = _span(a), _span(b)
     return a1 <= b0 or b1 <= a0
+
+
+_NORM_TENSORS = ("x", "branch", "gate", "labels", "shift", "scale", "out")
+_POST_TENSORS, _PRE_TENSORS = ("post weight", "post bias"), ("pre weight", "pre bias")
+_ROPE_TENSORS = ("q", "k", "positions", "q_weight", "k_weight", "out_q", "out_k")
+_INT4_TENSORS = ("x", "weight", "scales", "zeros", "bias")
 
 
 class NormSpec(NamedTuple):
@@ -587,8 +602,7 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
         raise ValueError("shift, scale and quantize belong to the pre-norm: give pre")
     if quantize and convrot and width % 256:
         raise ValueError("ConvRot256 needs a width that is a multiple of 256")
-    _inference("residual_norm", dev, x=x, branch=branch, gate=gate, labels=labels, shift=shift,
-               scale=scale, out=out)
+    _inference("residual_norm", dev, (x, branch, gate, labels, shift, scale, out), _NORM_TENSORS)
     if branch is None:
         if pre is None or post is not None or gate is not None or out is not None \
                 or residual_scale != 1.0:
@@ -599,7 +613,10 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
             raise ValueError(f"branch: {tuple(x.shape)} of {x.dtype} or fp32 required")
         branch = branch.contiguous()
         xo = x if out is None else _out(out, x.shape, x.dtype, dev, "out")
-        if not _apart(xo, branch) or (xo.data_ptr() != x.data_ptr() and not _apart(xo, x)):
+        # all three are contiguous: their addresses and sizes say whether they overlap
+        at, size = xo.data_ptr(), x.nbytes
+        b_at = branch.data_ptr()
+        if at < b_at + branch.nbytes and b_at < at + size or xo is not x and 0 < abs(at - x.data_ptr()) < size:
             raise ValueError("out must be x itself or overlap neither x nor the branch")
     rows = next((t.shape[0] for t in (gate, shift, scale)
                  if isinstance(t, torch.Tensor) and t.ndim == 2), 1)
@@ -615,9 +632,9 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
         lab = _need(labels, torch.int32, "labels", 1)
         if lab.numel() != M:
             raise ValueError("one label per row required")
-    for spec, name in ((post, "post"), (pre, "pre")):
+    for spec, names in ((post, _POST_TENSORS), (pre, _PRE_TENSORS)):
         if spec is not None:
-            _inference("residual_norm", dev, **{name + " weight": spec.weight, name + " bias": spec.bias})
+            _inference("residual_norm", dev, (spec.weight, spec.bias), names)
     pk, pw, pb, pe = _norm_args(post, width, "post")
     nk, nw, nb, ne = _norm_args(pre, width, "pre")
     h = q = s = None
@@ -633,7 +650,7 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
            kind if branch is None else _TYPES[branch.dtype], M, width, float(residual_scale),
            _ptr(g), g_ld, _ptr(sh), sh_ld, _ptr(sc), sc_ld, rows, _ptr(lab), pk, _ptr(pw), _ptr(pb),
            pe, nk, _ptr(nw), _ptr(nb), ne, _ptr(xo), _ptr(h), int(bool(convrot)), _ptr(q), _ptr(s),
-           _stream(x))
+           _raw_stream(dev))
     return x if xo is None else xo, q if quantize else h, s
 
 
@@ -700,8 +717,7 @@ def qk_norm_rope(q, k, positions, plan, *, q_weight=None, k_weight=None, eps: fl
         raise ValueError("eps must not be negative")
     if not norm and (q_weight is not None or k_weight is not None):
         q_weight = k_weight = None
-    _inference("qk_norm_rope", dev, q=q, k=k, positions=positions, q_weight=q_weight,
-               k_weight=k_weight, out_q=out_q, out_k=out_k)
+    _inference("qk_norm_rope", dev, (q, k, positions, q_weight, k_weight, out_q, out_k), _ROPE_TENSORS)
     positions = positions.contiguous()
     wq = None if q_weight is None else _vec(q_weight, D, "q_weight")
     wk = None if k_weight is None or k is None else _vec(k_weight, D, "k_weight")
@@ -711,13 +727,13 @@ def qk_norm_rope(q, k, positions, plan, *, q_weight=None, k_weight=None, eps: fl
     ok = None if k is None else _head_out(out_k, k, "out_k")
     if S == 0:
         return oq, ok
-    N.call("h3_qk_norm_rope", q.data_ptr(), q.stride(0), q.stride(1), hq, oq.data_ptr(),
-           oq.stride(0), oq.stride(1), _ptr(k), 0 if k is None else k.stride(0),
-           0 if k is None else k.stride(1), 0 if k is None else k.shape[1], _ptr(ok),
-           0 if k is None else ok.stride(0), 0 if k is None else ok.stride(1), S, D,
+    (qt, qh, _), (qot, qoh, _) = q.stride(), oq.stride()
+    (kt, kh, _), (kot, koh, _) = ((0, 0, 0),) * 2 if k is None else (k.stride(), ok.stride())
+    N.call("h3_qk_norm_rope", q.data_ptr(), qt, qh, hq, oq.data_ptr(), qot, qoh, _ptr(k), kt, kh,
+           0 if k is None else k.shape[1], _ptr(ok), kot, koh, S, D,
            _TYPES[q.dtype], positions.data_ptr(), _POSITIONS[positions.dtype], plan.n_axes,
            plan.turns, plan.axis, plan.pairs, plan.half, int(bool(norm)), _ptr(wq), _ptr(wk),
-           float(eps), _stream(q))
+           float(eps), _raw_stream(dev))
     return oq, ok
 
 
@@ -768,7 +784,7 @@ def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, o
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in (x.dtype, torch.float32):
         raise ValueError("out_dtype must be x's type or fp32")
-    _inference("int4_linear", x.device, x=x, weight=weight, scales=scales, zeros=zeros, bias=bias)
+    _inference("int4_linear", x.device, (x, weight, scales, zeros, bias), _INT4_TENSORS)
     if K > 1 and x.stride(1) != 1 or x.stride(0) < K:
         x = x.contiguous()
     scales = scales.contiguous()
@@ -779,7 +795,7 @@ def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, o
         return out
     N.call("h3_int4_linear", x.data_ptr(), _TYPES[x.dtype], x.stride(0) if M > 1 else K, M, K,
            weight.data_ptr(), n, scales.data_ptr(), _TYPES[scales.dtype], _ptr(zeros), group,
-           _ptr(b), out.data_ptr(), _TYPES[out_dtype], _stream(x))
+           _ptr(b), out.data_ptr(), _TYPES[out_dtype], _raw_stream(x.device))
     return out
 
 
