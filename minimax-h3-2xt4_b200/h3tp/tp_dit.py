@@ -404,3 +404,92 @@ class TPDiTLinearBlockINT8(nn.Module):
         # FC1 reads the updated residual (the norm is the identity here): a copy, since
         # the MLP updates x in place
         return mlp_forward(self.fc1, self.fc2, x, x.clone(), gate_mlp, segments)
+
+
+def _row_branch(module: RowParallelLinearINT8, x: torch.Tensor, input_act=None) -> torch.Tensor:
+    """A row projection's output for a norm behind it: the FP32 sum as the transport gives
+    it (residual_norm reads it as it is), or the fp16 forward where a LoRA adapter adds to it."""
+    if getattr(module, "lora_adapter", None) is not None:
+        return module(x, input_act=input_act)
+    _check_device_error(x)
+    from .h3_operator_policy import row_linear as dispatch_row
+    return dispatch_row(module, x, row_linear, module._comm(), input_act)
+
+
+class TPDiTModulatedBlockINT8(nn.Module):
+    """A DiT block on one TP rank with everything but attention: the modulation tables from
+    a 4-bit projection of the conditioning rows, RMS norms before and after both branches
+    joined with the gated residual, and QK norm with rotary positions on several axes
+    between the INT8 projections:
+
+        shift, scale, gate (twice) = modulation(cond)
+        codes        = quantise(norm(x) (1 + scale) + shift)       residual_norm
+        q, k, v      = turn(norm(qkv_proj(codes)))                 packed_qk_norm_rope, in place
+        x           += gate * norm(out_proj(attention(q, k, v)))   residual_norm, which also
+        codes        = quantise(norm(x) (1 + scale) + shift)       makes FC1's input
+        x           += gate * norm(fc2(swiglu(fc1(codes))))        residual_norm
+
+    heads counts the heads of all ranks, head_dim is the plan's; `attention` takes (q, k, v),
+    each [S, heads / world, head_dim] fp16 (views of one packed tensor), and returns
+    [S, heads / world, head_dim]; without one the values pass through.  Norm weights and the
+    modulation are replicated over the ranks."""
+
+    def __init__(self, hidden: int, ffn: int, heads: int, axes, cond_features: int, rank: int = 0,
+                 world_size: int = 1, device=None, policy=None, comm=None, eps: float = 1e-6,
+                 group: int = 128):
+        super().__init__()
+        from .h3_operator_policy import H3OperatorPolicy, configure_block
+        from .int4_linear import ColumnParallelLinearINT4
+        inner = heads * axes.head_dim
+        if heads % world_size or hidden % 256 or (inner // world_size) % 256:
+            raise ValueError("heads must divide by the ranks; hidden and a rank's heads * head_dim by 256")
+        self.hidden, self.heads, self.axes, self.eps = hidden, heads // world_size, axes, eps
+        self.modulation = ColumnParallelLinearINT4(cond_features, 6 * hidden, group=group, bias=True,
+                                                   out_dtype=torch.float32, device=device)
+        self.qkv_proj = ColumnParallelLinearINT8(hidden, 3 * inner, rank, world_size, components=3, device=device)
+        self.out_proj = RowParallelLinearINT8(inner, hidden, rank, world_size, device=device)
+        self.fc1 = ColumnParallelLinearINT8(hidden, 2 * ffn, rank, world_size, components=2, device=device)
+        self.fc2 = RowParallelLinearINT8(ffn, hidden, rank, world_size, device=device)
+        self.out_proj.comm = self.fc2.comm = comm
+
+        def ones(n):
+            return nn.Parameter(torch.ones(n, dtype=torch.float32, device=self.qkv_proj.weight.device),
+                                requires_grad=False)
+
+        self.attn_norm, self.attn_post_norm = ones(hidden), ones(hidden)
+        self.mlp_norm, self.mlp_post_norm = ones(hidden), ones(hidden)
+        self.q_norm, self.k_norm = ones(axes.head_dim), ones(axes.head_dim)
+        configure_block(self, "dit", policy or H3OperatorPolicy(fc1_swiglu_epilogue=True))
+
+    def forward(self, x: torch.Tensor, cond: torch.Tensor, positions: torch.Tensor, attention=None,
+                segments=None) -> torch.Tensor:
+        """x: fp16 residual [S, hidden], updated in place; cond: fp16 or bf16 [R, cond_features],
+        one row for each modulation row of `segments` (R 1: no segments needed); positions:
+        [S, axes]."""
+        from . import ops
+        from .dit_fusion import labels_for
+        from .rms_rope import packed_qk_norm_rope
+        labels = None
+        if cond.shape[0] != 1:
+            labels = labels_for(x, segments, cond.shape[0])
+            if labels is None:
+                raise ValueError("several modulation rows need segments that tile the rows exactly")
+
+        def norm(weight):
+            return ops.NormSpec("rms", weight, None, self.eps)
+
+        tables = self.modulation(cond).chunk(6, 1)
+        shift_a, scale_a, gate_a, shift_m, scale_m, gate_m = tables
+        _, codes, row_scale = ops.residual_norm(x, labels=labels, pre=norm(self.attn_norm), shift=shift_a,
+                                                scale=scale_a, quantize=True)
+        qkv = self.qkv_proj.forward_quantized(codes, row_scale)
+        q, k, v = packed_qk_norm_rope(qkv, self.heads, self.heads, positions, self.axes, q_weight=self.q_norm,
+                                      k_weight=self.k_norm, eps=self.eps)
+        out = v if attention is None else attention(q, k, v)
+        branch = _row_branch(self.out_proj, out.reshape(x.shape[0], -1).contiguous())
+        _, codes, row_scale = ops.residual_norm(x, branch, gate_a, labels, post=norm(self.attn_post_norm),
+                                                pre=norm(self.mlp_norm), shift=shift_m, scale=scale_m,
+                                                quantize=True)
+        branch = _row_branch(self.fc2, self.fc1.forward_quantized(codes, row_scale), "swiglu")
+        ops.residual_norm(x, branch, gate_m, labels, post=norm(self.mlp_post_norm))
+        return x

@@ -752,3 +752,118 @@ def test_int4_linear_refusals(cuda_device):
     r(x, w[:0], s[:0], z[:0])
     r(x[:, :0], w[:, :0], s[:, :0], z[:, :0])
     r(x.clone().requires_grad_(), w, s, z)
+
+
+# --------------------------------------------------------------------------------------
+# a block of them
+# --------------------------------------------------------------------------------------
+def _block(hidden, ffn, heads, axes, cond, seed):
+    from h3tp.tp_dit import TPDiTModulatedBlockINT8
+    g = _gen(seed)
+    block = TPDiTModulatedBlockINT8(hidden, ffn, heads, axes, cond, device="cuda", group=64)
+    for m in (block.qkv_proj, block.out_proj, block.fc1, block.fc2):
+        m.weight.data.copy_(torch.randint(-127, 128, m.weight.shape, generator=g, device="cuda", dtype=torch.int8))
+        m.weight_scale.data.copy_(torch.rand(m.weight_scale.shape, generator=g, device="cuda") * 2e-4 + 1e-4)
+    block.modulation.load_from_full(_randn(g, 6 * hidden, cond) * 0.05, _randn(g, 6 * hidden) * 0.2)
+    for w in (block.attn_norm, block.attn_post_norm, block.mlp_norm, block.mlp_post_norm, block.q_norm, block.k_norm):
+        w.data.copy_(1 + 0.1 * _randn(g, w.numel()))
+    return block, g
+
+
+def _dequantised(module, x):
+    """x through an INT8 projection's weights in 64 bits (the rotation is orthonormal and the
+    weights are stored rotated, so x is rotated and not the weights)."""
+    w = module.weight.double() * module.weight_scale.double()
+    return _rotate(x) @ w.T
+
+
+def _softmax_attention(q, k, v):
+    s = torch.einsum("shd,thd->hst", q.double(), k.double()) / q.shape[-1] ** 0.5
+    return torch.einsum("hst,thd->shd", s.softmax(-1), v.double())
+
+
+@pytest.mark.parametrize("rows,cond_rows", [(1, 1), (300, 3)])
+def test_modulated_block(cuda_device, rows, cond_rows):
+    """The whole block against its definition in 64 bits.  INT8 activations dominate: a code is
+    off by half a step, a step is 1/127 of the rotated row's maximum, about 4 of its standard
+    deviations, so each quantised activation carries an error of about (4 / 127) / sqrt(12) =
+    0.9% of its norm; four of them in a row, through norms that keep ratios, stay within 4 *
+    0.9% of the branches' norm, and twice that is allowed."""
+    from h3tp.rms_rope import RotaryAxes
+    axes = RotaryAxes(64, (16, 24, 24))
+    block, g = _block(512, 1024, 8, axes, 192, rows)
+    x = _randn(g, rows, 512).half()
+    cond = _randn(g, cond_rows, 192).half()
+    pos = _positions(g, rows, 3, "i32", far=64)
+    cuts = [0, rows // 3, rows // 2, rows]
+    segments = [(cuts[i], cuts[i + 1], i) for i in range(3)] if cond_rows > 1 else None
+    labels = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    for a, b, r in segments or []:
+        labels[a:b] = r
+    m = block.modulation
+    mods, _ = _int4_ref(cond, m.weight, m.weight_scale, None, 64, m.bias)
+    sa, ca, ga, sm, cm, gm = [t.contiguous() for t in mods.chunk(6, 1)]
+
+    def norm(v, w):
+        return v / (v.square().mean(-1, keepdim=True) + block.eps).sqrt() * w.double()
+
+    lab = labels.long()
+    h = norm(x.double(), block.attn_norm) * (1 + ca[lab]) + sa[lab]
+    q, k, v = _dequantised(block.qkv_proj, h).reshape(rows, 3, 8, 64).unbind(1)
+    q, _ = _rope_ref(q, block.q_norm, pos, axes, True, block.eps)
+    k, _ = _rope_ref(k, block.k_norm, pos, axes, True, block.eps)
+    y = _dequantised(block.out_proj, _softmax_attention(q, k, v).reshape(rows, 512))
+    want = x.double() + ga[lab] * norm(y, block.attn_post_norm)
+    h = norm(want, block.mlp_norm) * (1 + cm[lab]) + sm[lab]
+    gate, up = _dequantised(block.fc1, h).chunk(2, 1)
+    y = _dequantised(block.fc2, torch.nn.functional.silu(gate) * up)
+    delta = want - x.double() + gm[lab] * norm(y, block.mlp_post_norm)
+
+    before = x.clone()
+    out = block(x, cond, pos, lambda q, k, v: _softmax_attention(q, k, v).half(), segments)
+    assert out is x
+    got = out.double() - before.double()
+    assert torch.isfinite(out).all()
+    err = ((got - delta).norm() / delta.norm()).item()
+    assert err <= 0.072, err
+
+
+def test_modulated_block_captured(cuda_device):
+    """A captured block replayed on new inputs gives the bits of an eager one."""
+    from h3tp.rms_rope import RotaryAxes
+    axes = RotaryAxes(64, (16, 24, 24), pairing="half")
+    block, g = _block(512, 1024, 8, axes, 192, 5)
+    x0, cond = _randn(g, 640, 512).half(), _randn(g, 2, 192).half()
+    pos = _positions(g, 640, 3, "i32")
+    segments = [(0, 77, 0), (77, 640, 1)]
+    x = x0.clone()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        block(x, cond, pos, segments=segments)
+    torch.cuda.current_stream().wait_stream(st)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        block(x, cond, pos, segments=segments)
+    for i in range(2):
+        cond.mul_(0.5)
+        x.copy_(x0 * (i + 1))
+        gr.replay()
+        y = x0 * (i + 1)
+        block(y, cond, pos, segments=segments)
+        assert torch.equal(x, y)
+
+
+def test_modulated_block_refusals(cuda_device):
+    from h3tp.rms_rope import RotaryAxes
+    from h3tp.tp_dit import TPDiTModulatedBlockINT8
+    axes = RotaryAxes(64, (64,))
+    _refused(TPDiTModulatedBlockINT8, 500, 1024, 8, axes, 192, device="cuda")
+    _refused(TPDiTModulatedBlockINT8, 512, 1024, 6, axes, 192, device="cuda")
+    _refused(TPDiTModulatedBlockINT8, 512, 1024, 9, axes, 192, world_size=2, device="cuda")
+    block, g = _block(512, 1024, 8, axes, 192, 6)
+    x, cond = torch.zeros(4, 512, dtype=torch.float16, device="cuda"), _randn(g, 2, 192).half()
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    _refused(block, x, cond, pos)
+    _refused(block, x, cond, pos, segments=[(0, 3, 0)])
+    _refused(block, x, cond[:1], pos[:3])
