@@ -139,7 +139,7 @@ H3_DEV void tile_barrier(int id, int warps) {
 }
 
 // A CTA takes MT * 8 rows of x and, in rounds, wn tiles of 16 columns; its 16 warps are wn
-// tiles by 16 / wn slices of k (every (16 / wn)-th stage), whose sums are added in order
+// tiles by 16 / wn slices of k (rounded down; every (16 / wn)-th stage), whose sums are added in order
 // through shared memory at the end of a round.  A warp's stages of all rounds are one
 // sequence, fetched kStages - 1 ahead.  Where x of all of k fits, it is staged once.
 // GB: 32-k blocks of a group.  VEC: rows of packed weights start on 16-byte boundaries (k a
@@ -152,10 +152,11 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int WN = a.wn, WK = kInt4Warps / WN;
-  const int wn = warp % WN, wk = warp / WN;
+  const int stages = (a.k + kStageK - 1) / kStageK;
+  // warps beyond wn * wk have no slice: they only help to stage x
+  const int wn = warp % WN, wk = warp / WN < WK ? warp / WN : stages + WK;
   const int64_t m0 = (int64_t)blockIdx.y * kRows;
   const int rows = (int)min((int64_t)kRows, a.m - m0);
-  const int stages = (a.k + kStageK - 1) / kStageK;
   const int tiles = (a.n + 15) / 16, rounds = (tiles + WN * (int)gridDim.x - 1) / (WN * (int)gridDim.x);
   // staged x: the rows that exist and one of zeros for those that do not, in 16-byte units of
   // the eight values of a word's codes.  At one step the lanes of a row read every GB-th unit,
@@ -357,26 +358,28 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
 
     // the slices' sums through shared memory, added in order; then bias and store.  Only the
     // warps of one tile wait for one another.
-    float* const tile = sums + wn * WK * rows * 16;
+    if (wk < WK) {
+      float* const tile = sums + wn * WK * rows * 16;
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
+      for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = j * 8 + 2 * t + (i & 1);
-        if (row < rows) tile[(wk * rows + row) * 16 + g + (i >> 1) * 8] = acc[j][i];
+        for (int i = 0; i < 4; ++i) {
+          const int row = j * 8 + 2 * t + (i & 1);
+          if (row < rows) tile[(wk * rows + row) * 16 + g + (i >> 1) * 8] = acc[j][i];
+        }
+      tile_barrier(1 + wn, WK);
+      for (int i = wk * 32 + lane; i < rows * 16; i += WK * 32) {
+        const int n = n0 + (i & 15), row = i >> 4;
+        if (n >= a.n) continue;
+        float v = 0.0f;
+        for (int q = 0; q < WK; ++q) v += tile[q * rows * 16 + i];
+        if (a.bias != nullptr) v += __ldg(a.bias + n);
+        const int64_t at = (m0 + row) * a.n + n;
+        if (a.out_type == H3_TYPE_F32) reinterpret_cast<float*>(a.out)[at] = v;
+        else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
       }
-    tile_barrier(1 + wn, WK);
-    for (int i = wk * 32 + lane; i < rows * 16; i += WK * 32) {
-      const int n = n0 + (i & 15), row = i >> 4;
-      if (n >= a.n) continue;
-      float v = 0.0f;
-      for (int q = 0; q < WK; ++q) v += tile[q * rows * 16 + i];
-      if (a.bias != nullptr) v += __ldg(a.bias + n);
-      const int64_t at = (m0 + row) * a.n + n;
-      if (a.out_type == H3_TYPE_F32) reinterpret_cast<float*>(a.out)[at] = v;
-      else reinterpret_cast<T*>(a.out)[at] = from_f32<T>(v);
+      tile_barrier(1 + wn, WK);
     }
-    tile_barrier(1 + wn, WK);
   }
   cp_async_wait<0>();
 }
@@ -390,7 +393,7 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
   const int ctas = std::max(1, sms / blocks_m);
   int64_t best = -1;
-  for (int wn = 1; wn <= kInt4Warps; wn *= 2) {
+  for (int wn = 1; wn <= kInt4Warps; ++wn) {
     const int wk = kInt4Warps / wn;
     // in quarters of a stage; joining slices costs about as much as one stage
     const int64_t cost = (int64_t)((tiles + wn * ctas - 1) / (wn * ctas)) *
@@ -404,7 +407,10 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   const int rows = (int)std::min<int64_t>(8 * MT, a.m);
   const int fixed = kInt4Warps * (kStages * kStageBytes + rows * 16 * (int)sizeof(float));
   const int all = stages * kStageK, room = (226 * 1024 - fixed) / (rows + 1) - 64;
-  a.chunk = std::min(all, room / 2 / kStageK * kStageK);
+  a.chunk = room / 2 / kStageK * kStageK;
+  if (a.chunk >= all) a.chunk = all;
+  else if (const int slices = kInt4Warps / a.wn * kStageK; a.chunk >= slices)
+    a.chunk -= a.chunk % slices;  // as many stages for every slice of k
   const int smem = fixed + (rows + 1) * (a.chunk * 2 + 64);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
