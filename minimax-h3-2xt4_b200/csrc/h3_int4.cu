@@ -42,6 +42,7 @@ struct Int4Args {
 constexpr int kInt4Warps = 16;
 constexpr int kStageK = 256;  // k of one stage of a warp
 constexpr int kStages = 3;
+constexpr int kInt4Smem = 226 * 1024;
 constexpr int kStageBytes = 16 * kStageK / 2;
 
 // (a & MASK) | b in one instruction, which takes one constant and not two.
@@ -139,7 +140,7 @@ H3_DEV void tile_barrier(int id, int warps) {
 }
 
 // A CTA takes MT * 8 rows of x and, in rounds, wn tiles of 16 columns; its 16 warps are wn
-// tiles by 16 / wn slices of k (rounded down; every (16 / wn)-th stage), whose sums are added in order
+// tiles by WK = 16 / wn slices of k (rounded down, at most the stages; every WK-th stage), whose sums are added in order
 // through shared memory at the end of a round.  A warp's stages of all rounds are one
 // sequence, fetched kStages - 1 ahead.  Where x of all of k fits, it is staged once.
 // GB: 32-k blocks of a group.  VEC: rows of packed weights start on 16-byte boundaries (k a
@@ -151,8 +152,8 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int WN = a.wn, WK = kInt4Warps / WN;
   const int stages = (a.k + kStageK - 1) / kStageK;
+  const int WN = a.wn, WK = min(kInt4Warps / WN, stages);
   // warps beyond wn * wk have no slice: they only help to stage x
   const int wn = warp % WN, wk = warp / WN < WK ? warp / WN : stages + WK;
   const int64_t m0 = (int64_t)blockIdx.y * kRows;
@@ -387,18 +388,20 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
 template <typename T, typename S, bool ZEROS, int MT, int GB, bool VEC>
 int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   auto kern = int4_kernel<T, S, ZEROS, MT, GB, VEC>;
-  // Column tiles at a time: the number that needs the fewest stages one after the other on
-  // the busiest SM.
+  // Column tiles at a time.  The busiest SM's time in stages: its warps' work, which about 12
+  // warps saturate, or the longest chain of one warp; and for each round the joining of the
+  // slices (1 x 5120 x 25600: 28 us as 12 tiles without slices, 33 as 4 tiles of 4 slices
+  // in 3 rounds, 44 as 1 of 16 in 11).
   const int stages = (a.k + kStageK - 1) / kStageK, tiles = (a.n + 15) / 16;
   const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
   const int ctas = std::max(1, sms / blocks_m);
-  int64_t best = -1;
+  float best = 0.0f;
   for (int wn = 1; wn <= kInt4Warps; ++wn) {
-    const int wk = kInt4Warps / wn;
-    // in quarters of a stage; joining slices costs about as much as one stage
-    const int64_t cost = (int64_t)((tiles + wn * ctas - 1) / (wn * ctas)) *
-                         (4 * ((stages + wk - 1) / wk) + (wk > 1 ? 4 : 1));
-    if (best < 0 || cost < best) {
+    const int wk = std::min(kInt4Warps / wn, stages);
+    const float rounds = (float)((tiles + wn * ctas - 1) / (wn * ctas));
+    const float work = rounds * (float)wn * (float)stages / 12.0f, chain = rounds * (float)((stages + wk - 1) / wk);
+    const float cost = std::max(work, chain) + rounds * (wk > 1 ? 1.5f : 0.3f);
+    if (wn == 1 || cost < best) {
       best = cost;
       a.wn = wn;
     }
@@ -406,10 +409,10 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   // x of all of k where it fits beside the weights' stages and the sums, else in chunks
   const int rows = (int)std::min<int64_t>(8 * MT, a.m);
   const int fixed = kInt4Warps * (kStages * kStageBytes + rows * 16 * (int)sizeof(float));
-  const int all = stages * kStageK, room = (226 * 1024 - fixed) / (rows + 1) - 64;
+  const int all = stages * kStageK, room = (kInt4Smem - fixed) / (rows + 1) - 64;
   a.chunk = room / 2 / kStageK * kStageK;
   if (a.chunk >= all) a.chunk = all;
-  else if (const int slices = kInt4Warps / a.wn * kStageK; a.chunk >= slices)
+  else if (const int slices = std::min(kInt4Warps / a.wn, stages) * kStageK; a.chunk >= slices)
     a.chunk -= a.chunk % slices;  // as many stages for every slice of k
   const int smem = fixed + (rows + 1) * (a.chunk * 2 + 64);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -427,7 +430,11 @@ int launch_int4_shape(Int4Args& a, int sms, cudaStream_t stream) {
     return a.m <= 8 ? launch_int4<T, S, ZEROS, 1, GB, false>(a, sms, stream)
                     : launch_int4<T, S, ZEROS, 4, GB, false>(a, sms, stream);
   if (a.m <= 8) return launch_int4<T, S, ZEROS, 1, GB, true>(a, sms, stream);
-  if (a.m <= 16) return launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream);
+  // 16 rows a CTA, or 32 where all of their x fits (32 x 12800 x 5120: 63 us as two blocks
+  // of 16 rows, 88 as one of 32 with two and a half times the chunks of x)
+  const int64_t rows = std::min<int64_t>(a.m, 32), x32 = (rows + 1) * (2 * (int64_t)a.k + 512 + 64);
+  if (a.m <= 16 || x32 + kInt4Warps * (kStages * kStageBytes + rows * 64) > kInt4Smem)
+    return launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream);
   return launch_int4<T, S, ZEROS, 4, GB, true>(a, sms, stream);
 }
 
