@@ -43,7 +43,10 @@ constexpr int kInt4Warps = 16;
 constexpr int kStageK = 256;  // k of one stage of a warp
 constexpr int kStages = 3;
 constexpr int kInt4Smem = 226 * 1024;
-constexpr int kStageBytes = 16 * kStageK / 2;
+// Bytes of a slot's row: the stage's, and for rows that do not start on 16-byte boundaries one
+// more 16-byte word, as the words around a row's part are fetched whole.
+template <bool VEC>
+constexpr int kSlotRow = kStageK / 2 + (VEC ? 0 : 16);
 
 // (a & MASK) | b in one instruction, which takes one constant and not two.
 template <uint32_t MASK>
@@ -144,11 +147,13 @@ H3_DEV void tile_barrier(int id, int warps) {
 // through shared memory at the end of a round.  A warp's stages of all rounds are one
 // sequence, fetched kStages - 1 ahead.  Where x of all of k fits, it is staged once.
 // GB: 32-k blocks of a group.  VEC: rows of packed weights start on 16-byte boundaries (k a
-// multiple of 32), so they are fetched by cp.async; else byte by byte.
+// multiple of 32); else the aligned words around a row's part are fetched and a lane shifts
+// its bytes out of them.
 template <typename T, typename S, bool ZEROS, int MT, int GB, bool VEC>
 __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_constant__ Int4Args a) {
   constexpr int kRows = 8 * MT;
   constexpr int kGroups = kStageK / 32 / GB;  // groups of a stage
+  constexpr int kRowBytes = kSlotRow<VEC>, kStageBytes = 16 * kRowBytes;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
   // A stage in its slot: 16 rows of 128 bytes, the 16-byte words of a row exchanged so that
   // the rows that one read of a quarter touches at once fill all banks.
   const auto exchanged = [](int row) { return GB == 4 ? (row & 1) << 2 : GB == 2 ? (row & 3) << 1 : row & 7; };
-  const int w_unit = GB == 4 ? t : GB == 2 ? t >> 1 : 0, w_byte = GB == 4 ? 0 : GB == 2 ? (t & 1) * 8 : t * 4;
+  const int w_unit = GB == 4 ? t : GB == 2 ? t >> 1 : 0, w_byte = !VEC || GB == 4 ? 0 : GB == 2 ? (t & 1) * 8 : t * 4;
 
   // the fetching side: stages wk, wk + WK, ... of this warp's tile of every round; rows
   // behind the last column are read as the last.  Behind a row's end a slot keeps any codes:
@@ -202,19 +207,26 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = i * 4 + (lane >> 3);
-            cp_async16((uint32_t)__cvta_generic_to_shared(dst + row * 128 + (((lane & 7) ^ exchanged(row)) << 4)),
+            cp_async16((uint32_t)__cvta_generic_to_shared(dst + row * kRowBytes + (((lane & 7) ^ exchanged(row)) << 4)),
                        f_src + (int64_t)min(row, last) * a.pitch + byte);
           }
         }
       } else {
-        for (int i = lane; i < 16 * kStageK / 8; i += 32) {
-          const int row = i / (kStageK / 8), word = i % (kStageK / 8), byte = f_stage * (kStageK / 2) + word * 4;
-          const uint8_t* src = f_src + (int64_t)min(row, last) * a.pitch + byte;
-          uint32_t v = 0;
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (byte + b < a.pitch) v |= (uint32_t)__ldg(src + b) << (8 * b);
-          *reinterpret_cast<uint32_t*>(dst + row * 128 + (((word >> 2) ^ exchanged(row)) << 4) + (word & 3) * 4) = v;
+        const uint8_t* const end = a.w + (int64_t)a.n * a.pitch;
+        const int left = min(kStageK / 2, a.pitch - f_stage * (kStageK / 2));  // bytes of the part
+#pragma unroll 1
+        for (int i = lane; i < 16 * 9; i += 32) {
+          const int row = i / 9, word = i - row * 9;
+          const uint8_t* src = f_src + (int64_t)min(row, last) * a.pitch + f_stage * (kStageK / 2);
+          const uint8_t* p = src - ((uintptr_t)src & 15) + word * 16;
+          uint8_t* to = dst + row * kRowBytes + word * 16;
+          if (p >= src + left) continue;
+          if (p >= a.w && p + 16 <= end) {
+            cp_async16((uint32_t)__cvta_generic_to_shared(to), p);
+          } else {  // the words over the tensor's own ends
+            for (int e = 0; e < 16; ++e)
+              if (p + e >= a.w && p + e < end) to[e] = p[e];
+          }
         }
       }
       f_stage += WK;
@@ -282,6 +294,13 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
           if (ZEROS) zero[r][q] = q < left ? __ldg(a.zeros + group0[r] + first + q) : (uint8_t)0;
         }
     };
+    // where the rows g and g + 8 start in their first words
+    int skew[2] = {0, 0};
+    if (!VEC) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        skew[r] = (int)((uintptr_t)(a.w + (int64_t)min(n0 + g + 8 * r, a.n - 1) * a.pitch) & 15);
+    }
     int s = wk;
     look(s);
     for (int k0 = 0; k0 < a.k; k0 += a.chunk) {
@@ -305,15 +324,28 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
         look(s + WK);
         cp_async_wait<kStages - 2>();
         __syncwarp();
-        const uint8_t* w_row = ring + slot * kStageBytes + g * 128 + w_byte;
+        const uint8_t* w_row = ring + slot * kStageBytes + g * kRowBytes + w_byte;
         const int x_at = (s * kStageK - k0) * 2;
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
           uint32_t w[2][GB];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
+            if (!VEC) {
+              const uint8_t* p = w_row + r * 8 * kRowBytes + skew[r] + (q * 4 + t) * 4 * GB;
+              const uint32_t* at = reinterpret_cast<const uint32_t*>(p - ((uintptr_t)p & 3));
+              const int shift = ((uintptr_t)p & 3) * 8;
+              uint32_t low = at[0];
+#pragma unroll
+              for (int i = 0; i < GB; ++i) {
+                const uint32_t high = at[i + 1];
+                w[r][i] = __funnelshift_r(low, high, shift);
+                low = high;
+              }
+              continue;
+            }
             // rows g and g + 8 are exchanged alike
-            const uint8_t* p = w_row + r * 1024 + (((q * GB + w_unit) ^ exchanged(g)) << 4);
+            const uint8_t* p = w_row + r * 8 * kRowBytes + (((q * GB + w_unit) ^ exchanged(g)) << 4);
             if (GB == 4) {
               const uint4 v = *reinterpret_cast<const uint4*>(p);
               w[r][0] = v.x; w[r][1 % GB] = v.y; w[r][2 % GB] = v.z; w[r][3 % GB] = v.w;
@@ -408,7 +440,7 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   }
   // x of all of k where it fits beside the weights' stages and the sums, else in chunks
   const int rows = (int)std::min<int64_t>(8 * MT, a.m);
-  const int fixed = kInt4Warps * (kStages * kStageBytes + rows * 16 * (int)sizeof(float));
+  const int fixed = kInt4Warps * (kStages * 16 * kSlotRow<VEC> + rows * 16 * (int)sizeof(float));
   const int all = stages * kStageK, room = (kInt4Smem - fixed) / (rows + 1) - 64;
   a.chunk = room / 2 / kStageK * kStageK;
   if (a.chunk >= all) a.chunk = all;
@@ -426,16 +458,17 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
 
 template <typename T, typename S, bool ZEROS, int GB>
 int launch_int4_shape(Int4Args& a, int sms, cudaStream_t stream) {
-  if (a.k % 32 != 0 || !h3host::aligned(a.w, 16))
-    return a.m <= 8 ? launch_int4<T, S, ZEROS, 1, GB, false>(a, sms, stream)
-                    : launch_int4<T, S, ZEROS, 4, GB, false>(a, sms, stream);
-  if (a.m <= 8) return launch_int4<T, S, ZEROS, 1, GB, true>(a, sms, stream);
+  const bool vec = a.k % 32 == 0 && h3host::aligned(a.w, 16);
+  if (a.m <= 8) return vec ? launch_int4<T, S, ZEROS, 1, GB, true>(a, sms, stream)
+                           : launch_int4<T, S, ZEROS, 1, GB, false>(a, sms, stream);
   // 16 rows a CTA, or 32 where all of their x fits (32 x 12800 x 5120: 63 us as two blocks
   // of 16 rows, 88 as one of 32 with two and a half times the chunks of x)
   const int64_t rows = std::min<int64_t>(a.m, 32), x32 = (rows + 1) * (2 * (int64_t)a.k + 512 + 64);
-  if (a.m <= 16 || x32 + kInt4Warps * (kStages * kStageBytes + rows * 64) > kInt4Smem)
-    return launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream);
-  return launch_int4<T, S, ZEROS, 4, GB, true>(a, sms, stream);
+  if (a.m <= 16 || x32 + kInt4Warps * (kStages * 16 * (vec ? kSlotRow<true> : kSlotRow<false>) + rows * 64) > kInt4Smem)
+    return vec ? launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream)
+               : launch_int4<T, S, ZEROS, 2, GB, false>(a, sms, stream);
+  return vec ? launch_int4<T, S, ZEROS, 4, GB, true>(a, sms, stream)
+             : launch_int4<T, S, ZEROS, 4, GB, false>(a, sms, stream);
 }
 
 template <typename T, typename S, bool ZEROS>
