@@ -58,6 +58,15 @@ int sm_count(int device) {
   return g_sm_count[device];
 }
 
+namespace {
+// Lets the calling thread make calls that a stream capture would otherwise forbid.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+}  // namespace
+
 // The error word of a device: one int of host-mapped, page-locked memory, written by
 // kernels with a system-scope store and read by the host directly (h3_device_error_peek
 // needs no synchronisation).  Created on first use with the device current.
@@ -65,6 +74,8 @@ int* error_word(int device) {
   if (device < 0 || device >= kMaxDevices) return nullptr;
   std::lock_guard<std::mutex> lock(g_mutex);
   if (g_error_word[device] == nullptr) {
+    // allowed while a stream of this thread is being captured: the word is no part of a graph
+    RelaxedCapture relaxed;
     int* host = nullptr;
     if (cudaHostAlloc(reinterpret_cast<void**>(&host), sizeof(int),
                       cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {

@@ -17,8 +17,13 @@
 // four takes the t-th quarter of each group's bytes in one read of 4, 8 or 16 bytes, and x,
 // staged in shared memory, is permuted to match the pairs that the unpacking of a 4-byte word
 // yields, (0, 4), (1, 5), (2, 6), (3, 7).  Weights come through cp.async, two stages ahead;
-// straight into registers they left too few bytes in flight (44 against 33 us at 9 x 5376 x
-// 32256).
+// loaded straight into registers, as far ahead as those allow, the same products took 44 us
+// against 38 (9 x 5376 x 32256, fp16, groups of 128).
+//
+// That case reads 92 MB, 14 us at the measured copy rate; the kernel needs 38 us (0.38), a
+// single row of 5120 x 25600 in groups of 64 with zeros 28 us (0.39): bound by the issue of
+// about 50 instructions for 16 x 32 weights, 18 of them the unpacking, with the logical ones
+// at half rate.
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -499,7 +504,7 @@ extern "C" int h3_int4_linear(const void* x, int x_type, int64_t x_ld, int64_t m
     return t == H3_TYPE_F32 || t == H3_TYPE_F16 || t == H3_TYPE_BF16;
   };
   if (x == nullptr || w == nullptr || scales == nullptr || out == nullptr || m < 0 ||
-      m > 32 * 65535 || k < 1 || n < 1 || x_ld < 0 || (m > 1 && x_ld < k) || k > (1 << 24) ||
+      m > 16 * 65535 || k < 1 || n < 1 || x_ld < 0 || (m > 1 && x_ld < k) || k > (1 << 24) ||
       n > (1 << 24) || (group != 32 && group != 64 && group != 128) || !type_ok(scale_type) ||
       (x_type != H3_TYPE_F16 && x_type != H3_TYPE_BF16) ||
       (out_type != H3_TYPE_F32 && out_type != x_type))

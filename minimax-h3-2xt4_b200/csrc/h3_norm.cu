@@ -12,6 +12,11 @@
 // norms' weights, four times the row's own bytes, are folded into three factors a value
 // and stay in registers until a row has another label, and rows to come are fetched by
 // cp.async into slots of shared memory that only the fetching thread reads.
+//
+// 32768 x 3072 fp16 with both norms, gate and h stored (805 MB): 178 us, 0.69 of the measured
+// copy rate; with codes of the rotated row instead of h (705 MB) 245 us, 0.44, the rotation's
+// shuffles and the quantiser filling the issue slots.  One row at a time and factors read
+// from memory, the second took 376 us.
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -547,7 +552,8 @@ __global__ void __launch_bounds__(ROWS == 1 ? 1024 : kPairThreads)
   cp_async_wait<0>();
 }
 
-// Wide rows (NC chunks a thread) and rows of any width and alignment (VEC false).
+// Wide rows (NC chunks a thread) and rows of any width and alignment (VEC false).  With one
+// chunk a thread the factors stay in registers (16384 x 4001 fp32: 355 us, 461 without).
 template <typename XT, typename BT, int NC, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_constant__ ResidualNorm a,
                                                                  const __grid_constant__ Deal d) {
@@ -556,9 +562,15 @@ __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_co
   bool in_row[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) in_row[c] = d.at(c, 0) < d.width;
+  Factors f;
+  int64_t held = -1;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t lab = row_label(a, a.labels != nullptr ? __ldg(a.labels + row) : 0);
     const int64_t base = row * a.width;
+    if (NC == 1 && lab != held) {
+      load_factors<VEC>(a, d, 0, in_row[0], lab, f);
+      held = lab;
+    }
     f32x2 v[1][NC][4];  // the branch, then x', then h
     if (a.branch != nullptr) {
 #pragma unroll
@@ -571,8 +583,7 @@ __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_co
       for (int c = 0; c < NC; ++c) {
         f32x2 x[4];
         load_chunk<XT, VEC>(reinterpret_cast<const XT*>(a.x) + base, d, c, in_row[c], x);
-        Factors f;
-        load_factors<VEC>(a, d, c, in_row[c], lab, f);
+        if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[0][c][i] = fma2(f.gate[i], v[0][c][i], mul2(x[i], rs));
         if (a.post_bias != nullptr) add_post_bias<VEC>(a, d, c, in_row[c], lab, v[0][c]);
@@ -587,8 +598,7 @@ __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_co
     normalise<1, NC, VEC>(v, a, d, in_row, a.pre_kind, a.pre_eps, reduce);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      Factors f;
-      load_factors<VEC>(a, d, c, in_row[c], lab, f);
+      if (NC > 1) load_factors<VEC>(a, d, c, in_row[c], lab, f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[0][c][i] = fma2(v[0][c][i], f.scale[i], f.shift[i]);
       if (!QUANT) store_chunk<XT, VEC>(reinterpret_cast<XT*>(a.h) + base, d, c, in_row[c], v[0][c]);

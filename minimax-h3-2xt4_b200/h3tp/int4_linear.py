@@ -92,8 +92,9 @@ class ColumnParallelLinearINT4(nn.Module):
                 continue
             held = getattr(self, name)
             part = self._rows(full)
-            if part.shape != held.shape or (name == "weight" and part.dtype != torch.uint8):
-                raise ValueError(f"{name}: {tuple(held.shape)} a rank required, got {tuple(part.shape)}")
+            if part.shape != held.shape or part.dtype != held.dtype:
+                raise ValueError(f"{name}: {held.dtype} {tuple(held.shape)} a rank required, got "
+                                 f"{part.dtype} {tuple(part.shape)}")
             held.data.copy_(part)
 
     def load_from_full(self, full_weight: torch.Tensor, bias=None):

@@ -867,3 +867,29 @@ def test_modulated_block_refusals(cuda_device):
     _refused(block, x, cond, pos)
     _refused(block, x, cond, pos, segments=[(0, 3, 0)])
     _refused(block, x, cond[:1], pos[:3])
+
+
+def test_first_labelled_call_in_a_capture(cuda_device):
+    """A process whose first call with labels is captured: the error word is made without
+    breaking the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from h3tp import ops
+x = torch.ones(5, 256, dtype=torch.float16, device="cuda")
+shift = torch.tensor([[0.0], [1.0]], device="cuda").expand(2, 256).contiguous()
+labels = torch.tensor([0, 1, 0, 1, 1], dtype=torch.int32, device="cuda")
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    _, h, _ = ops.residual_norm(x, labels=labels, pre=ops.NormSpec("rms", eps=0.0), shift=shift)
+graph.replay()
+torch.cuda.synchronize()
+assert h[:, 0].tolist() == [1.0, 2.0, 1.0, 2.0, 2.0], h[:, 0]
+"""
+    pkg = Path(__file__).resolve().parents[1] / "minimax-h3-2xt4_b200"
+    r = subprocess.run([sys.executable, "-c", code, str(pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
