@@ -408,6 +408,8 @@ H3_DEV void quantise(f32x2 (&v)[ROWS][NC][4], const ResidualNorm& a, const Deal&
   }
 }
 
+H3_DEV void prefetch_line(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 H3_DEV int64_t row_label(const ResidualNorm& a, int64_t lab) {
   if (lab >= 0 && lab < a.mod_rows) return lab;
   report_error(a.err, H3_ERR_INVALID);
@@ -553,7 +555,8 @@ __global__ void __launch_bounds__(ROWS == 1 ? 1024 : kPairThreads)
 }
 
 // Wide rows (NC chunks a thread) and rows of any width and alignment (VEC false).  With one
-// chunk a thread the factors stay in registers (16384 x 4001 fp32: 355 us, 461 without).
+// chunk a thread the factors stay in registers (16384 x 4001 fp32: 355 us, 461 without); the
+// CTA's next row is brought into the L2 (340 us).
 template <typename XT, typename BT, int NC, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_constant__ ResidualNorm a,
                                                                  const __grid_constant__ Deal d) {
@@ -567,6 +570,14 @@ __global__ void __launch_bounds__(1024) residual_norm_any_kernel(const __grid_co
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t lab = row_label(a, a.labels != nullptr ? __ldg(a.labels + row) : 0);
     const int64_t base = row * a.width;
+    if (row + gridDim.x < a.rows) {  // the CTA's next row, one line a thread
+      const int64_t next = (row + gridDim.x) * a.width;
+      for (int i = threadIdx.x * (128 / (int)sizeof(XT)); i < d.width; i += blockDim.x * (128 / (int)sizeof(XT)))
+        prefetch_line(reinterpret_cast<const XT*>(a.x) + next + i);
+      if (a.branch != nullptr)
+        for (int i = threadIdx.x * (128 / (int)sizeof(BT)); i < d.width; i += blockDim.x * (128 / (int)sizeof(BT)))
+          prefetch_line(reinterpret_cast<const BT*>(a.branch) + next + i);
+    }
     if (NC == 1 && lab != held) {
       load_factors<VEC>(a, d, 0, in_row[0], lab, f);
       held = lab;

@@ -10,8 +10,8 @@
 // shuffle tree over those lanes.  Each lane keeps up to 64 bytes of the heads to come in flight
 // through cp.async into slots of shared memory that it alone reads: held in registers,
 // the same bytes left too few warps an SM to cover the memory's latency (158 against
-// 143 us).  32768 tokens of 24 + 24 heads of 128 in fp16, 805 MB: 143 us, 5.6 TB/s, 0.86 of
-// the measured copy rate.
+// 143 us).  32768 tokens of 24 + 24 heads of 128 in fp16, 805 MB: 140 us, 5.7 TB/s, 0.88 of
+// the measured copy rate (halves paired: 156 us).
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas)
       weigh<T, HALF, true>(a, v.weight, u, c, s, t);
       const int64_t out_step = (int64_t)a.parts * v.out_head;
       T* out = reinterpret_cast<T*>(v.out) + r.token * v.out_token + (int64_t)r.part * v.out_head;
-#pragma unroll 1
+#pragma unroll 2
       for (int h = 0; h < steps; ++h) {
         cp_async_wait<kSlots - 2>();
         f32x2 x[4] = {0, 0, 0, 0};
