@@ -893,3 +893,68 @@ assert h[:, 0].tolist() == [1.0, 2.0, 1.0, 2.0, 2.0], h[:, 0]
     pkg = Path(__file__).resolve().parents[1] / "minimax-h3-2xt4_b200"
     r = subprocess.run([sys.executable, "-c", code, str(pkg)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("width", [32, 64, 1280, 2056, 5376, 6144, 6400])
+@pytest.mark.parametrize("xt,bt", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_residual_norm_many_rows_equal_few(cuda_device, width, xt, bt, kind):
+    """Enough rows for the kernel that takes two at a time, an odd number of them, labels that
+    change inside a pair, and a row with an infinity beside a finite one: the bits of the same
+    rows in small calls."""
+    from h3tp import ops
+    g = _gen(width)
+    rows = 741
+    x, b, gate, shift, scale, lab = _norm_case(g, rows, width, xt, bt, 3)
+    b[600] = float("inf")
+    spec = ops.NormSpec(kind, _randn(g, width), _randn(g, width))
+    quants = (False, True) if width % 256 == 0 else (False,)
+    for quant in quants:
+        kw = dict(post=spec, pre=spec, shift=shift, scale=scale, quantize=quant, residual_scale=0.5)
+        whole = ops.residual_norm(x.clone(), b, gate, lab, **kw)
+        first = ops.residual_norm(x, pre=spec, labels=lab, shift=shift, scale=scale, quantize=quant)
+        for at in range(0, rows, 137):
+            part = slice(at, at + 137)
+            few = ops.residual_norm(x[part].clone(), b[part], gate, lab[part], **kw)
+            alone = ops.residual_norm(x[part], pre=spec, labels=lab[part], shift=shift, scale=scale, quantize=quant)
+            for a, w in ((few, whole), (alone, first)):
+                for u, v in zip(a, w):
+                    assert u is None or torch.equal(torch.nan_to_num(u.float(), 7.0), torch.nan_to_num(v[part].float(), 7.0))
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("xt", ["f16", "f32"])
+def test_qk_norm_rope_many_tokens_equal_few(cuda_device, half, xt):
+    """More tokens than the GPU holds lane groups for: the bits of the same tokens in small
+    calls, whose heads are split, and in place on packed rows."""
+    from h3tp.rms_rope import RotaryAxes, packed_qk_norm_rope, qk_norm_rope
+    for dim, axes in ((64, (16, 24, 24)), (80, (40, 40)), (33, (8, 6, 10))):
+        plan = RotaryAxes(dim, axes, pairing="half" if half else "interleaved")
+        g = _gen(dim)
+        S, H, K = 25013, 3, 2
+        qkv = _randn(g, S, (H + 2 * K) * dim).to(DT[xt])
+        pos = _positions(g, S, len(axes), "i32")
+        wq, wk = _randn(g, dim), _randn(g, dim)
+        q = qkv[:, :H * dim].unflatten(1, (H, dim))
+        k = qkv[:, H * dim:(H + K) * dim].unflatten(1, (K, dim))
+        oq, ok = qk_norm_rope(q, k, pos, plan, q_weight=wq, k_weight=wk)
+        _close(oq, *_rope_ref(q, wq, pos, plan, True, 1e-6), ROPE_DEPTH)
+        _close(ok, *_rope_ref(k, wk, pos, plan, True, 1e-6), ROPE_DEPTH)
+        for at in range(0, S, 6007):
+            part = slice(at, at + 6007)
+            fq, fk = qk_norm_rope(q[part], k[part], pos[part], plan, q_weight=wq, k_weight=wk)
+            assert torch.equal(fq, oq[part]) and torch.equal(fk, ok[part])
+        pq, pk, _ = packed_qk_norm_rope(qkv, H, K, pos, plan, q_weight=wq, k_weight=wk)
+        assert torch.equal(pq, oq) and torch.equal(pk, ok)
+
+
+@pytest.mark.parametrize("m,k,n,group", [(3, 512, 40000, 32), (20, 300, 50001, 64), (32, 4096, 20000, 128),
+                                         (32, 4099, 20000, 64)])
+def test_int4_linear_many_columns(cuda_device, m, k, n, group):
+    """Several rounds of column tiles a CTA, with x held whole and in chunks."""
+    from h3tp import ops
+    g = _gen(n)
+    x, w, s, z = _int4_inputs(g, m, k, n, "f16", group, True, "f16")
+    bias = _randn(g, n)
+    y = ops.int4_linear(x, w, s, z, group=group, bias=bias, out_dtype=torch.float32)
+    _close(y, *_int4_ref(x, w, s, z, group, bias), _int4_depth(k, group))
