@@ -378,11 +378,16 @@ H3_DEV void quantise(f32x2 (&v)[ROWS][NC][4], const ResidualNorm& a, const Deal&
     for (int c = 0; c < NC; ++c) {
       uint32_t code[8];
       if (finite[r]) {
+        // the correctly rounded quotient (div_by_scale's correction of v * inv), as the library's
+        // other quantisers take it: v * inv alone falls to the other side of a border between
+        // codes once in about two million values (32768 x 3072 fp16: 244 us with it alone, 250 so).
         // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
         // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
+        const f32x2 i2 = dup2(inv), ns = dup2(-scale);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x2 t = fma2(v[r][c][i], dup2(inv), dup2(12582912.0f));
+          const f32x2 q0 = mul2(v[r][c][i], i2);
+          const f32x2 t = add2(fma2(fma2(q0, ns, v[r][c][i]), i2, q0), dup2(12582912.0f));
           code[i] = __float_as_uint(lo2(t));
           code[i + 4] = __float_as_uint(hi2(t));
         }
