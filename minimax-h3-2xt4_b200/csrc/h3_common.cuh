@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/h3b200.h"
 
@@ -507,6 +508,22 @@ int check_launch();                                  // maps cudaGetLastError to
 // one row with the 128-byte swizzle (row staging of the activation producers).
 bool encode_row_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes,
                     int box_lines);
+
+// Once per kernel and device (`allowed`: the kernel's own, one entry a device): raises the
+// kernel's limit of dynamic shared memory on the current device to `bytes`, the most that any
+// of its launches asks for.  The limit is shared by every thread of the process, so one
+// launch must not set it to its own size: it could fall between another thread's set and launch.
+constexpr int kMaxDevices = 64;
+template <typename K>
+bool allow_smem(K kernel, int bytes, int device, std::atomic<bool> (&allowed)[kMaxDevices]) {
+  if (allowed[device].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  allowed[device].store(true, std::memory_order_release);
+  return true;
+}
 
 inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p % a) == 0; }
 

@@ -9,7 +9,6 @@
 namespace h3host {
 
 namespace {
-constexpr int kMaxDevices = 64;
 std::mutex g_mutex;
 int g_sm_count[kMaxDevices] = {0};
 int* g_error_word[kMaxDevices] = {nullptr};  // device view of the mapped word

@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kInt4Warps * 32, 1) int4_kernel(const __grid_c
 }
 
 template <typename T, typename S, bool ZEROS, int MT, int GB, bool VEC>
-int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
+int launch_int4(Int4Args& a, int dev, cudaStream_t stream) {
   auto kern = int4_kernel<T, S, ZEROS, MT, GB, VEC>;
   // Column tiles at a time.  The busiest SM's time in stages: its warps' work, which about 12
   // warps saturate, or the longest chain of one warp; and for each round the joining of the
@@ -431,7 +431,7 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   // in 3 rounds, 44 as 1 of 16 in 11).
   const int stages = (a.k + kStageK - 1) / kStageK, tiles = (a.n + 15) / 16;
   const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
-  const int ctas = std::max(1, sms / blocks_m);
+  const int ctas = std::max(1, h3host::sm_count(dev) / blocks_m);
   float best = 0.0f;
   for (int wn = 1; wn <= kInt4Warps; ++wn) {
     const int wk = std::min(kInt4Warps / wn, stages);
@@ -452,45 +452,43 @@ int launch_int4(Int4Args& a, int sms, cudaStream_t stream) {
   else if (const int slices = std::min(kInt4Warps / a.wn, stages) * kStageK; a.chunk >= slices)
     a.chunk -= a.chunk % slices;  // as many stages for every slice of k
   const int smem = fixed + (rows + 1) * (a.chunk * 2 + 64);
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return H3_ERR_CUDA;
-  }
+  static std::atomic<bool> allowed[h3host::kMaxDevices];
+  if (!h3host::allow_smem(kern, kInt4Smem, dev, allowed)) return H3_ERR_CUDA;
   const dim3 grid(std::min(ctas, (tiles + a.wn - 1) / a.wn), blocks_m);
   kern<<<grid, kInt4Warps * 32, smem, stream>>>(a);
   return h3host::check_launch();
 }
 
 template <typename T, typename S, bool ZEROS, int GB>
-int launch_int4_shape(Int4Args& a, int sms, cudaStream_t stream) {
+int launch_int4_shape(Int4Args& a, int dev, cudaStream_t stream) {
   const bool vec = a.k % 32 == 0 && h3host::aligned(a.w, 16);
-  if (a.m <= 8) return vec ? launch_int4<T, S, ZEROS, 1, GB, true>(a, sms, stream)
-                           : launch_int4<T, S, ZEROS, 1, GB, false>(a, sms, stream);
+  if (a.m <= 8) return vec ? launch_int4<T, S, ZEROS, 1, GB, true>(a, dev, stream)
+                           : launch_int4<T, S, ZEROS, 1, GB, false>(a, dev, stream);
   // 16 rows a CTA, or 32 where all of their x fits (32 x 12800 x 5120: 63 us as two blocks
   // of 16 rows, 88 as one of 32 with two and a half times the chunks of x)
   const int64_t rows = std::min<int64_t>(a.m, 32), x32 = (rows + 1) * (2 * (int64_t)a.k + 512 + 64);
   if (a.m <= 16 || x32 + kInt4Warps * (kStages * 16 * (vec ? kSlotRow<true> : kSlotRow<false>) + rows * 64) > kInt4Smem)
-    return vec ? launch_int4<T, S, ZEROS, 2, GB, true>(a, sms, stream)
-               : launch_int4<T, S, ZEROS, 2, GB, false>(a, sms, stream);
-  return vec ? launch_int4<T, S, ZEROS, 4, GB, true>(a, sms, stream)
-             : launch_int4<T, S, ZEROS, 4, GB, false>(a, sms, stream);
+    return vec ? launch_int4<T, S, ZEROS, 2, GB, true>(a, dev, stream)
+               : launch_int4<T, S, ZEROS, 2, GB, false>(a, dev, stream);
+  return vec ? launch_int4<T, S, ZEROS, 4, GB, true>(a, dev, stream)
+             : launch_int4<T, S, ZEROS, 4, GB, false>(a, dev, stream);
 }
 
 template <typename T, typename S, bool ZEROS>
-int launch_int4_group(Int4Args& a, int group, int sms, cudaStream_t stream) {
-  if (group == 32) return launch_int4_shape<T, S, ZEROS, 1>(a, sms, stream);
-  if (group == 64) return launch_int4_shape<T, S, ZEROS, 2>(a, sms, stream);
-  return launch_int4_shape<T, S, ZEROS, 4>(a, sms, stream);
+int launch_int4_group(Int4Args& a, int group, int dev, cudaStream_t stream) {
+  if (group == 32) return launch_int4_shape<T, S, ZEROS, 1>(a, dev, stream);
+  if (group == 64) return launch_int4_shape<T, S, ZEROS, 2>(a, dev, stream);
+  return launch_int4_shape<T, S, ZEROS, 4>(a, dev, stream);
 }
 
 template <typename T>
-int launch_int4_type(Int4Args& a, int group, int sms, cudaStream_t stream) {
+int launch_int4_type(Int4Args& a, int group, int dev, cudaStream_t stream) {
   const bool z = a.zeros != nullptr;
   if (a.scale_type == H3_TYPE_F32)
-    return z ? launch_int4_group<T, uint32_t, true>(a, group, sms, stream)
-             : launch_int4_group<T, uint32_t, false>(a, group, sms, stream);
-  return z ? launch_int4_group<T, uint16_t, true>(a, group, sms, stream)
-           : launch_int4_group<T, uint16_t, false>(a, group, sms, stream);
+    return z ? launch_int4_group<T, uint32_t, true>(a, group, dev, stream)
+             : launch_int4_group<T, uint32_t, false>(a, group, dev, stream);
+  return z ? launch_int4_group<T, uint16_t, true>(a, group, dev, stream)
+           : launch_int4_group<T, uint16_t, false>(a, group, dev, stream);
 }
 
 }  // namespace h3
@@ -517,7 +515,6 @@ extern "C" int h3_int4_linear(const void* x, int x_type, int64_t x_ld, int64_t m
              (int)((k + 1) / 2), scale_type, out_type, 0, 0,
              h3host::aligned(x, 16) && (m == 1 || x_ld % 8 == 0)};
   cudaStream_t st = (cudaStream_t)stream;
-  const int sms = h3host::sm_count(dev);
-  return x_type == H3_TYPE_F16 ? launch_int4_type<__half>(a, group, sms, st)
-                               : launch_int4_type<__nv_bfloat16>(a, group, sms, st);
+  return x_type == H3_TYPE_F16 ? launch_int4_type<__half>(a, group, dev, st)
+                               : launch_int4_type<__nv_bfloat16>(a, group, dev, st);
 }

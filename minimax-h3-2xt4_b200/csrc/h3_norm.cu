@@ -22,6 +22,7 @@
 namespace h3 {
 
 constexpr int kPairThreads = 768;  // most threads of a CTA that takes two rows: 80 registers each
+constexpr int kRingSmem = 200 * 1024;  // most shared memory of a CTA's slots
 
 struct ResidualNorm {
   const void* x;
@@ -627,11 +628,10 @@ template <typename XT, typename BT, bool BRANCH, bool QUANT, int ROWS, int SLOTS
 int launch_ring(const ResidualNorm& a, const Deal& d, int threads, int dev, cudaStream_t stream) {
   auto kern = residual_norm_kernel<XT, BT, BRANCH, QUANT, ROWS, SLOTS>;
   const size_t smem = (size_t)SLOTS * ROWS * threads * 8 * (sizeof(XT) + (BRANCH ? sizeof(BT) : 0));
+  static std::atomic<bool> allowed[h3host::kMaxDevices];
   if (smem > 40 * 1024 &&  // with the static part, more than a launch may ask for unasked
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    cudaGetLastError();
+      !h3host::allow_smem(kern, kRingSmem, dev, allowed))
     return H3_ERR_CUDA;
-  }
   // CTAs an SM: what its registers and its shared memory hold
   const int by_regs = 65536 / ((ROWS == 1 ? 64 : 80) * threads), by_smem = (int)(220 * 1024 / (smem + 2048));
   const int ctas = std::max(1, std::min(std::min(by_regs, by_smem), 16));
@@ -651,7 +651,7 @@ int launch_norm_shape(const ResidualNorm& a, bool vec, int dev, cudaStream_t str
     // Two rows at a time where the registers allow it, there are rows for every SM to have
     // several pairs, and three slots of a pair fit; else one row, in four slots or two.
     const int64_t pair = 2ll * threads * 8 * (sizeof(XT) + (BRANCH ? sizeof(BT) : 0));
-    if (threads <= kPairThreads && a.rows >= 4ll * h3host::sm_count(dev) && 3 * pair <= 200 * 1024)
+    if (threads <= kPairThreads && a.rows >= 4ll * h3host::sm_count(dev) && 3 * pair <= kRingSmem)
       return launch_ring<XT, BT, BRANCH, QUANT, 2, 3>(a, d, threads, dev, stream);
     if (4 * pair / 2 <= 100 * 1024)
       return launch_ring<XT, BT, BRANCH, QUANT, 1, 4>(a, d, threads, dev, stream);

@@ -1,5 +1,7 @@
 """GPU tests of the operators around a block's projections beyond one call's agreement with its
 definition: codes against the library's other quantisers' rule, calls that meet other calls."""
+import threading
+
 import pytest
 import torch
 
@@ -33,3 +35,81 @@ def test_codes_are_the_rounded_quotient(cuda_device, rows, width):
     want = torch.round(h / s).clamp(-128, 127).to(torch.int8)
     wrong = int((q != want).sum())
     assert wrong == 0, (wrong, q.numel())
+
+
+# --------------------------------------------------------------------------------------
+# two sizes of one kernel at once: they ask for different amounts of shared memory
+# --------------------------------------------------------------------------------------
+def _int4_entry(k):
+    """A call of h3_int4_linear on a stream of its own, as a thread makes it: without Python's
+    own work around the entry point, two threads are inside it most of the time."""
+    from h3tp import _native as N
+    x = _randn(k, 8, k).half()
+    w = torch.randint(0, 256, (16, k // 2), device="cuda", dtype=torch.uint8)
+    s, out, st = torch.ones(16, k // 64, device="cuda"), torch.empty(8, 16, device="cuda"), torch.cuda.Stream()
+    args = (x.data_ptr(), N.TYPE_F16, k, 8, k, w.data_ptr(), 16, s.data_ptr(), N.TYPE_F32, None, 64, None,
+            out.data_ptr(), N.TYPE_F32, st.cuda_stream)
+    entry = N.load().h3_int4_linear
+    return lambda: entry(*args), (x, w, s, out, st)
+
+
+def _norm_entry(width):
+    from h3tp import _native as N
+    x, b = _randn(width, 8, width), _randn(width + 1, 8, width)
+    out, h, st = torch.empty_like(x), torch.empty_like(x), torch.cuda.Stream()
+    args = (x.data_ptr(), N.TYPE_F32, b.data_ptr(), N.TYPE_F32, 8, width, 1.0, None, 0, None, 0, None, 0, 1, None,
+            N.NORM_NONE, None, None, 0.0, N.NORM_RMS, None, None, 1e-6, out.data_ptr(), h.data_ptr(), 0, None, None,
+            st.cuda_stream)
+    entry = N.load().h3_residual_norm
+    return lambda: entry(*args), (x, b, out, h, st)
+
+
+@pytest.mark.parametrize("entry,big,small", [(_int4_entry, 8192, 256), (_norm_entry, 2944, 1536)],
+                         ids=["int4_linear", "residual_norm"])
+def test_two_threads_with_two_sizes(cuda_device, entry, big, small):
+    """Neither thread's launches are refused because of the other's size."""
+    calls = [entry(size) for size in (big, small)]
+    torch.cuda.synchronize()
+    refused = [0, 0]
+
+    def work(i):
+        for _ in range(20000):
+            refused[i] += calls[i][0]() != 0
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert refused == [0, 0]
+
+
+def test_graph_of_two_sizes(cuda_device):
+    """One graph with the larger size of a kernel before the smaller one, replayed."""
+    from h3tp import ops
+
+    def calls():
+        out = []
+        for k in (8192, 256):
+            x = _randn(k, 8, k).half()
+            w = torch.full((16, k // 2), 0x3A, device="cuda", dtype=torch.uint8)
+            s = torch.ones(16, k // 64, device="cuda")
+            out.append(([x], lambda x=x, w=w, s=s: ops.int4_linear(x, w, s, group=64)))
+        for width in (2944, 1536):
+            x, b = _randn(width, 8, width), _randn(width + 1, 8, width)
+            out.append(([x, b], lambda x=x, b=b: ops.residual_norm(x, b, pre=ops.NormSpec(), out=torch.empty_like(x))[1]))
+        return out
+
+    made = calls()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = [c() for _, c in made]
+    for _ in range(2):
+        for inputs, _ in made:
+            for t in inputs:
+                t.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(h, c()) for h, (_, c) in zip(held, made))
