@@ -443,6 +443,8 @@ class TPDiTModulatedBlockINT8(nn.Module):
         inner = heads * axes.head_dim
         if heads % world_size or hidden % 256 or (inner // world_size) % 256:
             raise ValueError("heads must divide by the ranks; hidden and a rank's heads * head_dim by 256")
+        # one device for the sharded projections and for what every rank holds whole
+        device = torch.device(device) if device is not None else torch.device("cuda", rank)
         self.hidden, self.heads, self.axes, self.eps = hidden, heads // world_size, axes, eps
         self.modulation = ColumnParallelLinearINT4(cond_features, 6 * hidden, group=group, bias=True,
                                                    out_dtype=torch.float32, device=device)
@@ -453,8 +455,7 @@ class TPDiTModulatedBlockINT8(nn.Module):
         self.out_proj.comm = self.fc2.comm = comm
 
         def ones(n):
-            return nn.Parameter(torch.ones(n, dtype=torch.float32, device=self.qkv_proj.weight.device),
-                                requires_grad=False)
+            return nn.Parameter(torch.ones(n, dtype=torch.float32, device=device), requires_grad=False)
 
         self.attn_norm, self.attn_post_norm = ones(hidden), ones(hidden)
         self.mlp_norm, self.mlp_post_norm = ones(hidden), ones(hidden)
