@@ -15,6 +15,15 @@ import torch.nn as nn
 from . import ops
 
 
+def _stored_scales(scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """fp32 scales in the type they are kept in, none of them 0.  Below fp16's normal numbers they
+    are rounded up to its steps of 2^-24: rounded down, a scale would cut its largest weights off."""
+    if dtype == torch.float16:
+        step = 2.0 ** -24
+        scales = torch.where(scales < torch.finfo(dtype).tiny, (scales / step).ceil().clamp(min=1) * step, scales)
+    return scales.clamp(min=torch.finfo(torch.float32).tiny).to(dtype)
+
+
 def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = False,
                   scale_dtype: torch.dtype = torch.float32):
     """Rounds a weight [N, K] to 4-bit codes with one scale for each group along K.
@@ -31,13 +40,12 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = Fa
     N, K = weight.shape
     groups = -(-K // group)
     w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group - K)).unflatten(1, (groups, group))
-    tiny = torch.finfo(torch.float32 if scale_dtype == torch.bfloat16 else scale_dtype).tiny
     if zero_points:
         lo, hi = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
-        scales = ((hi - lo) / 15).clamp(min=tiny).to(scale_dtype)
+        scales = _stored_scales((hi - lo) / 15, scale_dtype)
         zeros = torch.round(-lo / scales.float()).clamp(0, 15)
     else:
-        scales = (w.abs().amax(2) / 7).clamp(min=tiny).to(scale_dtype)
+        scales = _stored_scales(w.abs().amax(2) / 7, scale_dtype)
         zeros = None
     offset = 8.0 if zeros is None else zeros[:, :, None]
     code = torch.round(w / scales.float()[:, :, None] + offset).clamp(0, 15)

@@ -1,0 +1,34 @@
+"""Calls of the operators around a block's projections that the layout and refusal tests do not
+make, as far as they need no GPU."""
+import pytest
+import torch
+
+
+# --------------------------------------------------------------------------------------
+# 4-bit quantisation
+# --------------------------------------------------------------------------------------
+def _dequantised(packed, scales, zeros, k, group):
+    code = torch.stack((packed & 15, packed >> 4), 2).flatten(1)[:, :k].double()
+    zero = 8.0 if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
+    return (code - zero) * scales.double().repeat_interleave(group, 1)[:, :k]
+
+
+@pytest.mark.parametrize("magnitude", [1.0, 3e-4, 8e-6, 4e-7, 1e-8])
+@pytest.mark.parametrize("scale_dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_quantize_int4_of_small_weights(magnitude, scale_dtype, zero_points):
+    """Whatever the weights' magnitude, the scale follows them as far as its type reaches (fp16: in
+    steps of 2^-24 at the lowest) and a weight is off by half a scale: its code's rounding, and
+    with zero points the border codes' by what the scale's rounding moves 15 of it."""
+    from h3tp.int4_linear import quantize_int4
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(40, 200, generator=g) * magnitude
+    packed, s, z = quantize_int4(w, 64, zero_points, scale_dtype)
+    padded = torch.nn.functional.pad(w, (0, 56)).unflatten(1, (4, 64)).double()
+    span = padded.amax(2).clamp(min=0) - padded.amin(2).clamp(max=0) if zero_points else padded.abs().amax(2)
+    want = span / (15 if zero_points else 7)
+    eps = torch.finfo(scale_dtype).eps
+    step = 2.0 ** -24 if scale_dtype == torch.float16 else 0.0
+    assert ((s.double() - want).abs() <= want * (eps / 2 + 2.0 ** -22) + step).all()
+    off = (_dequantised(packed, s, z, 200, 64) - w.double()).abs()
+    assert (off <= s.double().repeat_interleave(64, 1)[:, :200] * (0.5 + 16 * (eps / 2 + 2.0 ** -22))).all()

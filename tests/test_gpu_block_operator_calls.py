@@ -113,3 +113,22 @@ def test_graph_of_two_sizes(cuda_device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(h, c()) for h, (_, c) in zip(held, made))
+
+
+# --------------------------------------------------------------------------------------
+# int4_linear: the smallest scales
+# --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,low", [(torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -126)])
+def test_scales_below_the_normal_numbers(cuda_device, dtype, low):
+    """fp16 scales down to the smallest subnormal, bf16 ones down to the smallest normal number:
+    x, codes and scales are small integers times a power of two here, so every sum is exact."""
+    from h3tp import ops
+    k, n = 128, 32
+    x = torch.randint(-8, 9, (3, k), device="cuda").to(torch.bfloat16)
+    codes = torch.randint(0, 16, (n, k), device="cuda")
+    w = (codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8)
+    steps = torch.randint(1, 8, (n, k // 64), device="cuda")
+    s = (steps.double() * low).to(dtype)
+    want = x.double() @ ((codes - 8).double() * steps.repeat_interleave(64, 1).double()).T * low
+    y = ops.int4_linear(x, w, s, group=64, out_dtype=torch.float32)
+    assert torch.equal(y.double(), want)
