@@ -21,7 +21,10 @@ def _stored_scales(scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     if dtype == torch.float16:
         step = 2.0 ** -24
         scales = torch.where(scales < torch.finfo(dtype).tiny, (scales / step).ceil().clamp(min=1) * step, scales)
-    return scales.clamp(min=torch.finfo(torch.float32).tiny).to(dtype)
+    stored = scales.clamp(min=torch.finfo(torch.float32).tiny).to(dtype)
+    if not torch.isfinite(stored).all():
+        raise ValueError(f"weight: not finite, or beyond what scales of {dtype} reach")
+    return stored
 
 
 def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = False,
@@ -30,19 +33,22 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = Fa
 
     Symmetric (zero_points False): W = scale * (code - 8), scale = max|W| / 7 of the
     group.  With zero points: W = scale * (code - zero), the range [min(W, 0), max(W, 0)]
-    over 15 steps.  The codes are chosen for the scales as stored (scale_dtype).
+    over 15 steps.  The codes are chosen for the scales as stored (scale_dtype); weights
+    that no finite scale of that type spans are refused.
     Returns (packed uint8 [N, ceil(K / 2)], scales [N, ceil(K / group)], zeros or None),
     as ops.int4_linear takes them, on the weight's device."""
     if weight.ndim != 2 or not weight.is_floating_point() or min(weight.shape) < 1:
         raise ValueError("weight: floating [N, K] required")
     if group not in ops.INT4_GROUPS:
         raise ValueError(f"group must be one of {ops.INT4_GROUPS}")
+    if scale_dtype not in ops._TYPES:
+        raise ValueError("scale_dtype must be fp32, fp16 or bf16")
     N, K = weight.shape
     groups = -(-K // group)
     w = torch.nn.functional.pad(weight.detach().float(), (0, groups * group - K)).unflatten(1, (groups, group))
     if zero_points:
         lo, hi = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
-        scales = _stored_scales((hi - lo) / 15, scale_dtype)
+        scales = _stored_scales(hi / 15 - lo / 15, scale_dtype)
         zeros = torch.round(-lo / scales.float()).clamp(0, 15)
     else:
         scales = _stored_scales(w.abs().amax(2) / 7, scale_dtype)

@@ -32,3 +32,25 @@ def test_quantize_int4_of_small_weights(magnitude, scale_dtype, zero_points):
     assert ((s.double() - want).abs() <= want * (eps / 2 + 2.0 ** -22) + step).all()
     off = (_dequantised(packed, s, z, 200, 64) - w.double()).abs()
     assert (off <= s.double().repeat_interleave(64, 1)[:, :200] * (0.5 + 16 * (eps / 2 + 2.0 ** -22))).all()
+
+
+@pytest.mark.parametrize("w,scale_dtype,zero_points", [
+    (float("nan"), torch.float32, False), (float("inf"), torch.float32, False), (float("-inf"), torch.bfloat16, True),
+    (5e5, torch.float16, False), (1.1e6, torch.float16, True), (1.0, torch.float64, False), (1.0, torch.int32, False)])
+def test_quantize_int4_refuses_what_scales_cannot_hold(w, scale_dtype, zero_points):
+    """A group that no finite scale of the type spans would come back as NaN."""
+    from h3tp.int4_linear import quantize_int4
+    full = torch.ones(2, 64)
+    full[1, 40] = w
+    with pytest.raises(ValueError):
+        quantize_int4(full, 32, zero_points, scale_dtype)
+
+
+def test_quantize_int4_at_the_ends_of_the_range():
+    from h3tp.int4_linear import quantize_int4
+    for w, dtype in ((4.5e5, torch.float16), (3.4e38, torch.float32), (3.3e38, torch.bfloat16)):
+        for zero_points in (False, True):
+            packed, s, z = quantize_int4(torch.tensor([[w, -w, 0.0, w / 3]]), 32, zero_points, dtype)
+            got = _dequantised(packed, s, z, 4, 32)
+            assert torch.isfinite(s.float()).all()
+            assert (got - torch.tensor([[w, -w, 0.0, w / 3]]).double()).abs().max() <= 0.6 * s.double().max()
