@@ -93,37 +93,39 @@ class ColumnParallelLinearINT4(nn.Module):
 
     def _rows(self, full):
         """This rank's rows of every component of a full tensor."""
+        rows = self.out_features_per_rank * self.world_size
+        if full.ndim < 1 or full.shape[0] != rows:
+            raise ValueError(f"{rows} rows over all ranks required, got {tuple(full.shape)}")
         parts = full.chunk(self.components, 0)
         return torch.cat([p.chunk(self.world_size, 0)[self.rank] for p in parts], 0)
+
+    def _load(self, **given):
+        """Copies this rank's parts into the parameters, after all of them were checked."""
+        parts = {name: part for name, part in given.items() if part is not None}
+        for name, part in parts.items():
+            held = getattr(self, name)
+            if part.shape != held.shape or part.dtype != held.dtype:
+                raise ValueError(f"{name}: {held.dtype} {tuple(held.shape)} a rank required, got "
+                                 f"{part.dtype} {tuple(part.shape)}")
+        for name, part in parts.items():
+            getattr(self, name).data.copy_(part)
 
     def load_quantized(self, packed, scales, zeros=None, bias=None):
         """Loads this rank's rows of a full quantised weight (quantize_int4's three results)."""
         if (zeros is None) != (self.weight_zero is None) or (bias is None) != (self.bias is None):
             raise ValueError("zero points and bias must be given exactly where the module holds them")
-        for name, full in (("weight", packed), ("weight_scale", scales), ("weight_zero", zeros),
-                           ("bias", bias)):
-            if full is None:
-                continue
-            held = getattr(self, name)
-            part = self._rows(full)
-            if part.shape != held.shape or part.dtype != held.dtype:
-                raise ValueError(f"{name}: {held.dtype} {tuple(held.shape)} a rank required, got "
-                                 f"{part.dtype} {tuple(part.shape)}")
-            held.data.copy_(part)
+        self._load(weight=self._rows(packed), weight_scale=self._rows(scales),
+                   weight_zero=None if zeros is None else self._rows(zeros),
+                   bias=None if bias is None else self._rows(bias))
 
     def load_from_full(self, full_weight: torch.Tensor, bias=None):
         """Quantises this rank's rows of a full floating weight and loads them."""
-        rows = self._rows(full_weight)
-        packed, scales, zeros = quantize_int4(rows, self.group, self.weight_zero is not None,
+        if (bias is None) != (self.bias is None):
+            raise ValueError("a bias must be given exactly where the module holds one")
+        packed, scales, zeros = quantize_int4(self._rows(full_weight), self.group, self.weight_zero is not None,
                                               self.weight_scale.dtype)
-        if packed.shape != self.weight.shape or (bias is None) != (self.bias is None):
-            raise ValueError("weight or bias does not fit the module")
-        self.weight.data.copy_(packed)
-        self.weight_scale.data.copy_(scales)
-        if zeros is not None:
-            self.weight_zero.data.copy_(zeros)
-        if bias is not None:
-            self.bias.data.copy_(self._rows(bias))
+        self._load(weight=packed, weight_scale=scales, weight_zero=zeros,
+                   bias=None if bias is None else self._rows(bias).float())
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         y = ops.int4_linear(x.reshape(-1, self.in_features), self.weight, self.weight_scale,

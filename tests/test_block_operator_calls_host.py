@@ -54,3 +54,39 @@ def test_quantize_int4_at_the_ends_of_the_range():
             got = _dequantised(packed, s, z, 4, 32)
             assert torch.isfinite(s.float()).all()
             assert (got - torch.tensor([[w, -w, 0.0, w / 3]]).double()).abs().max() <= 0.6 * s.double().max()
+
+
+# --------------------------------------------------------------------------------------
+# the 4-bit module's loaders
+# --------------------------------------------------------------------------------------
+def _module(rank=0, world=1, components=1, zero_points=False, bias=True):
+    from h3tp.int4_linear import ColumnParallelLinearINT4
+    return ColumnParallelLinearINT4(64, 12, rank, world, 32, zero_points=zero_points, bias=bias, device="cpu",
+                                    components=components)
+
+
+def _quantised(n, zero_points=False):
+    from h3tp.int4_linear import quantize_int4
+    return quantize_int4(torch.linspace(-1, 1, n * 64).reshape(n, 64), 32, zero_points)
+
+
+def test_int4_loaders_take_whole_tensors_only():
+    """A bias of one value is not spread over the rows, and tensors of another number of rows than
+    the module's are refused even where a rank's share of them would fit."""
+    full, bias = torch.ones(12, 64), torch.arange(12.0)
+    m = _module()
+    m.load_from_full(full, bias)
+    assert torch.equal(m.bias.data, bias)
+    packed, scales, _ = _quantised(12)
+    for bad in (torch.ones(1), torch.ones(12, 1), torch.ones(13), torch.tensor(1.0)):
+        with pytest.raises(ValueError):
+            m.load_from_full(full, bad)
+        with pytest.raises(ValueError):
+            m.load_quantized(packed, scales, None, bad)
+    assert torch.equal(m.bias.data, bias)  # nothing was loaded by a refused call
+    for rank, rows in ((1, 13), (0, 11), (1, 14)):  # chunks of 7 + 6, 6 + 5 and 7 + 7 rows
+        m = _module(rank, 2, bias=False)
+        with pytest.raises(ValueError):
+            m.load_from_full(torch.ones(rows, 64))
+        with pytest.raises(ValueError):
+            m.load_quantized(*_quantised(rows)[:2])
