@@ -451,9 +451,9 @@ int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int64_t q_he
  *   y[m][n] = sum_g scales[n][g] * sum_{k in g} x[m][k] (code[n][k] - zero[n][g]) + bias[n]
  * x: F16 or BF16 rows x_ld elements apart; w: [n][ceil(k / 2)] bytes, code k in the low
  * nibble of byte k / 2 for even k, in the high one for odd k; scales: [n][ceil(k / group)]
- * of scale_type; zeros: the same shape in bytes (0 to 15), or NULL for 8 everywhere; bias
- * may be NULL; out: [m][n] of x_type or F32.  group 32, 64 or 128.  Products of codes and
- * x are exact; sums are fp32. */
+ * of scale_type; zeros: the same shape in bytes (0 to 15, not checked; larger ones give
+ * wrong products), or NULL for 8 everywhere; bias may be NULL; out: [m][n] of x_type or
+ * F32.  group 32, 64 or 128.  Products of codes and x are exact; sums are fp32. */
 int h3_int4_linear(const void* x, int x_type, int64_t x_ld, int64_t m, int64_t k,
                    const uint8_t* w, int64_t n, const void* scales, int scale_type,
                    const uint8_t* zeros, int group, const float* bias, void* out, int out_type,

@@ -114,6 +114,8 @@ class ColumnParallelLinearINT4(nn.Module):
         """Loads this rank's rows of a full quantised weight (quantize_int4's three results)."""
         if (zeros is None) != (self.weight_zero is None) or (bias is None) != (self.bias is None):
             raise ValueError("zero points and bias must be given exactly where the module holds them")
+        if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+            raise ValueError("zero points must lie between 0 and 15")
         self._load(weight=self._rows(packed), weight_scale=self._rows(scales),
                    weight_zero=None if zeros is None else self._rows(zeros),
                    bias=None if bias is None else self._rows(bias))

@@ -764,7 +764,9 @@ def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, o
 
     weight: contiguous uint8 [N, ceil(K / 2)], code k in the low nibble of byte k // 2 for
     even k and in the high one for odd k; scales: fp32, fp16 or bf16 [N, ceil(K / group)];
-    zeros: uint8 of the same shape (0 to 15), None for 8 everywhere; bias: fp32 [N].
+    zeros: uint8 of the same shape, None for 8 everywhere; bias: fp32 [N].  Zero points must
+    lie between 0 and 15: the call does not read them on the host and larger ones give wrong
+    products (ColumnParallelLinearINT4's loader refuses them).
     Meant for few rows (a token or a handful): the weight is read once for every 32 rows."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.ndim != 2 \
             or x.dtype not in (torch.float16, torch.bfloat16):

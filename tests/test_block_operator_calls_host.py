@@ -90,3 +90,15 @@ def test_int4_loaders_take_whole_tensors_only():
             m.load_from_full(torch.ones(rows, 64))
         with pytest.raises(ValueError):
             m.load_quantized(*_quantised(rows)[:2])
+
+
+def test_int4_loader_refuses_zero_points_above_15():
+    m = _module(zero_points=True, bias=False)
+    packed, scales, zeros = _quantised(12, True)
+    m.load_quantized(packed, scales, zeros)
+    assert torch.equal(m.weight_zero.data, zeros)
+    bad = zeros.clone()
+    bad[7, 1] = 16
+    with pytest.raises(ValueError):
+        m.load_quantized(packed, scales, bad)
+    assert torch.equal(m.weight_zero.data, zeros)
