@@ -415,10 +415,11 @@ int h3_column_linear_noalloc_error(int device, int* code);
  * NULL.  gate / shift / scale: fp32 rows of `width` values, *_ld elements apart; NULL
  * reads as 1, 0 and 0.  x, out and h have x_type (F32, F16 or BF16); branch has it
  * too, or is F32.  out may be x (each thread writes what it read) and must not
- * otherwise overlap an input.  Exactly one of h and (q, row_scale) is written when
- * pre_kind is not NONE: h rounded once to x_type, or the INT8 codes and row scale of h
- * (rotated by ConvRot256 when convrot; width % 256 == 0 then).  Without a branch (NULL,
- * out NULL, no gate, no post norm, residual_scale 1) only the pre-norm runs.
+ * otherwise overlap an input (over a table, weight or the labels: H3_ERR_INVALID).
+ * Exactly one of h and (q, row_scale) is written when pre_kind is not NONE: h rounded
+ * once to x_type, or the INT8 codes and row scale of h (rotated by ConvRot256 when
+ * convrot; width % 256 == 0 then).  Without a branch (NULL, out NULL, no gate, no post
+ * norm, residual_scale 1) only the pre-norm runs.
  * width <= 32768; statistics and everything between the two roundings in fp32. */
 int h3_residual_norm(const void* x, int x_type, const void* branch, int branch_type,
                      int64_t rows, int64_t width, float residual_scale, const float* gate,
@@ -436,7 +437,8 @@ int h3_residual_norm(const void* x, int x_type, const void* branch, int branch_t
  * pair p is (p, p + pairs) when half, else (2p, 2p + 1); elements from 2 * pairs on are
  * normed and not turned.  Tensors are [tokens][heads][head_dim] of `type` with token and
  * head strides in elements and unit stride inside a head; an output may be its own
- * input (same pointer and strides) and must not otherwise overlap an input.  positions:
+ * input (same pointer and strides) and must not otherwise overlap an input (heads of
+ * an output over positions or a weight: H3_ERR_INVALID).  positions:
  * [tokens][axes] int32, int64 or fp32 (pos_kind).  turns (double) and axis are HOST
  * arrays of `pairs` entries, copied before the call returns.  head_dim <= 256. */
 int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int64_t q_heads,

@@ -525,6 +525,16 @@ bool allow_smem(K kernel, int bytes, int device, std::atomic<bool> (&allowed)[kM
   return true;
 }
 
+// Whether one of `rows` rows of `row` bytes, `step` bytes apart from p on, has a byte in the
+// `bytes` bytes from `from` on.  Gaps between the rows do not count; nothing is at nullptr.
+inline bool rows_meet(const void* p, int64_t rows, int64_t row, int64_t step, const void* from, int64_t bytes) {
+  const int64_t at = (int64_t)(uintptr_t)p, first = (int64_t)(uintptr_t)from, last = first + bytes;
+  if (p == nullptr || from == nullptr || bytes <= 0 || at >= last) return false;
+  if (at + row > first) return true;
+  const int64_t r = step > 0 ? (first - at - row) / step + 1 : rows;  // the first row that ends behind `first`
+  return r < rows && at + r * step < last;
+}
+
 inline bool aligned(const void* p, unsigned a) { return ((uintptr_t)p % a) == 0; }
 
 }  // namespace h3host

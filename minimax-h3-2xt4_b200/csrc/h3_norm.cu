@@ -706,6 +706,14 @@ extern "C" int h3_residual_norm(const void* x, int x_type, const void* branch, i
       (quant && convrot && width % 256 != 0))
     return H3_ERR_INVALID;
   if (rows == 0) return H3_OK;
+  // every row reads the tables, weights and labels: x' must lie over none of them
+  const auto over = [&](const void* p, int64_t n, int64_t ld) {
+    return h3host::rows_meet(p, n, width * 4, ld * 4, out, rows * width * (x_type == H3_TYPE_F32 ? 4 : 2));
+  };
+  if (over(gate, mod_rows, gate_ld) || over(shift, mod_rows, shift_ld) || over(scale, mod_rows, scale_ld) ||
+      over(post_weight, 1, 0) || over(post_bias, 1, 0) || over(pre_weight, 1, 0) || over(pre_bias, 1, 0) ||
+      h3host::rows_meet(labels, 1, rows * 4, 0, out, rows * width * (x_type == H3_TYPE_F32 ? 4 : 2)))
+    return H3_ERR_INVALID;
   int dev;
   h3host::DeviceScope scope;
   if (int s = scope.bind(x, &dev)) return s;

@@ -435,6 +435,17 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
     if (a.axis[p] >= axes) return H3_ERR_INVALID;
   }
   if (tokens == 0) return H3_OK;
+  // every head reads its token's positions and the weights: no output may lie over them
+  const int64_t size = type == H3_TYPE_F32 ? 4 : 2;
+  for (const HeadView* v : {&a.q, &a.k}) {
+    const auto over = [&](const void* p, int64_t bytes) {  // over a token's heads, from first to last
+      const int64_t heads = size * ((v->heads - 1) * (int64_t)v->out_head + head_dim);
+      return p != nullptr && h3host::rows_meet(v->out, tokens, heads, size * v->out_token, p, bytes);
+    };
+    if (over(positions, tokens * axes * (pos_kind == H3_POS_I64 ? 8 : 4)) || over(q_weight, head_dim * 4) ||
+        over(k_weight, head_dim * 4))
+      return H3_ERR_INVALID;
+  }
   int dev;
   h3host::DeviceScope scope;
   if (int s = scope.bind(q, &dev)) return s;

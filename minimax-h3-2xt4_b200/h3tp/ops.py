@@ -587,7 +587,8 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
 
     gate, shift, scale: fp32 tables [R, N], all of the same R (slices of one wider table
     are read in place); labels: int32 [M], needed unless R is 1.  A label out of range
-    reads row 0 and sets the device error word.
+    reads row 0 and sets the device error word.  x' must not lie over a table, a norm's
+    weight or the labels: every row reads those (refused).
 
     Returns (x', h or codes or None, row_scale [M, 1] or None)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.ndim != 2 or x.dtype not in _TYPES:

@@ -132,3 +132,46 @@ def test_scales_below_the_normal_numbers(cuda_device, dtype, low):
     want = x.double() @ ((codes - 8).double() * steps.repeat_interleave(64, 1).double()).T * low
     y = ops.int4_linear(x, w, s, group=64, out_dtype=torch.float32)
     assert torch.equal(y.double(), want)
+
+
+# --------------------------------------------------------------------------------------
+# outputs over tables, weights and positions
+# --------------------------------------------------------------------------------------
+def test_outputs_may_not_overlap_what_is_read(cuda_device):
+    """Every row reads the tables and weights, so an output over one of them is refused; between
+    the rows of a table there is room for one."""
+    from h3tp import ops
+    from h3tp.rms_rope import RotaryAxes, qk_norm_rope
+    pre = ops.NormSpec()
+    buf = _randn(1, 6, 64)
+    x, b = buf[2:5], torch.ones(3, 64, device="cuda")
+    lab = torch.zeros(3, dtype=torch.int32, device="cuda")
+    one, keep = torch.zeros(1, 64, device="cuda"), buf.clone()
+    for bad in (dict(gate=buf[2:3]), dict(gate=buf[1:3], labels=lab), dict(pre=pre, shift=buf[4:5]),
+                dict(pre=pre, scale=buf[4:], labels=lab), dict(pre=ops.NormSpec("rms", buf[3])),
+                dict(pre=ops.NormSpec("rms", None, buf[3])), dict(post=ops.NormSpec("rms", buf[4])),
+                dict(post=ops.NormSpec("layer", None, buf[2])),
+                dict(gate=one, labels=buf.view(torch.int32).view(-1)[130:133])):
+        with pytest.raises(ValueError):
+            ops.residual_norm(x, b, **bad)
+        with pytest.raises(ValueError):
+            ops.residual_norm(x.clone(), b, out=x, **bad)
+    assert torch.equal(buf, keep)
+    ops.residual_norm(x, b, gate=buf[1:2], pre=ops.NormSpec("rms", buf[5]), shift=buf[:1])
+    wide = _randn(2, 2, 128)
+    ops.residual_norm(wide[:1, 64:], b[:1], gate=wide[:, :64], labels=lab[:1])  # x between the gate's rows
+
+    axes = RotaryAxes(64, (64,))
+    packed = _randn(3, 4, 3, 64)
+    q, pos = packed[:, :1], torch.zeros(4, dtype=torch.int32, device="cuda")
+    whole = packed[:, :2]
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, None, pos, axes, q_weight=packed[1, 0], out_q=q)
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, whole[:, 1:], pos, axes, k_weight=packed[2, 1], out_k=whole[:, 1:])
+    with pytest.raises(ValueError):
+        qk_norm_rope(q, None, packed.view(torch.int32).view(-1)[:4], axes, out_q=q)
+    w = packed[1, 2]  # between the heads of two tokens
+    want, _ = qk_norm_rope(q.clone(), None, pos, axes, q_weight=w.clone())
+    qk_norm_rope(q, None, pos, axes, q_weight=w, out_q=q)
+    assert torch.equal(q, want)
