@@ -130,6 +130,8 @@ class ColumnParallelLinearINT4(nn.Module):
                    bias=None if bias is None else self._rows(bias).float())
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.ndim < 1 or x.shape[-1] != self.in_features:
+            raise ValueError(f"x: in_features {self.in_features} required, got {tuple(x.shape)}")
         y = ops.int4_linear(x.reshape(-1, self.in_features), self.weight, self.weight_scale,
                             self.weight_zero, group=self.group, bias=self.bias,
                             out_dtype=self.out_dtype)

@@ -102,3 +102,14 @@ def test_int4_loader_refuses_zero_points_above_15():
     with pytest.raises(ValueError):
         m.load_quantized(packed, scales, bad)
     assert torch.equal(m.weight_zero.data, zeros)
+
+
+# --------------------------------------------------------------------------------------
+# arguments that are no tensors, inputs of another width
+# --------------------------------------------------------------------------------------
+def test_int4_module_refuses_other_widths():
+    """Rows are not cut anew to the module's width."""
+    m = _module()
+    for shape in ((3, 32), (2, 128), (64, 3), (128,), ()):
+        with pytest.raises(ValueError, match="in_features|64"):
+            m(torch.zeros(shape, dtype=torch.float16))
