@@ -500,11 +500,13 @@ def _raw_stream(device: torch.device) -> int:
 
 
 def _inference(where: str, device, tensors, names) -> None:
-    """Every tensor on `device`, none that autograd would have to follow."""
+    """Everything given is a tensor on `device`, none that autograd would have to follow."""
     grad = torch.is_grad_enabled()
     for t, name in zip(tensors, names):
         if t is None:
             continue
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name}: tensor required")
         if t.device != device:
             raise ValueError(f"{name}: on {t.device}, the call runs on {device}")
         if grad and t.requires_grad:
@@ -635,6 +637,8 @@ def residual_norm(x, branch=None, gate=None, labels=None, *, post: Optional[Norm
             raise ValueError("one label per row required")
     for spec, names in ((post, _POST_TENSORS), (pre, _PRE_TENSORS)):
         if spec is not None:
+            if not isinstance(spec, NormSpec):
+                raise ValueError("post and pre: NormSpec or None required")
             _inference("residual_norm", dev, (spec.weight, spec.bias), names)
     pk, pw, pb, pe = _norm_args(post, width, "post")
     nk, nw, nb, ne = _norm_args(pre, width, "pre")
@@ -702,12 +706,14 @@ def qk_norm_rope(q, k, positions, plan, *, q_weight=None, k_weight=None, eps: fl
     h3tp.rms_rope documents the arguments.  Returns (q', k')."""
     _heads(q, "q")
     dev, (S, hq, D) = q.device, q.shape
+    if not hasattr(plan, "head_dim"):
+        raise ValueError("plan: RotaryAxes required")
     if D != plan.head_dim:
         raise ValueError(f"q: head_dim {plan.head_dim} of the plan required, got {D}")
-    if hq < 1 or (k is not None and k.ndim == 3 and k.shape[1] < 1):
-        raise ValueError("at least one head required")
     if k is not None:
         _heads(k, "k", q)
+    if hq < 1 or (k is not None and k.shape[1] < 1):
+        raise ValueError("at least one head required")
     if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITIONS:
         raise ValueError("positions: int32, int64 or fp32 tensor required")
     if positions.ndim == 1 and plan.n_axes == 1:
@@ -775,19 +781,19 @@ def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, o
     M, K = x.shape
     if group not in INT4_GROUPS:
         raise ValueError(f"group must be one of {INT4_GROUPS}")
-    if weight.dtype != torch.uint8 or weight.ndim != 2 or not weight.is_contiguous() or K < 1 \
+    _inference("int4_linear", x.device, (x, weight, scales, zeros, bias), _INT4_TENSORS)
+    if weight is None or weight.dtype != torch.uint8 or weight.ndim != 2 or not weight.is_contiguous() or K < 1 \
             or weight.shape[0] < 1 or weight.shape[1] != (K + 1) // 2:
         raise ValueError(f"weight: contiguous uint8 [N, {(K + 1) // 2}] required")
     n = weight.shape[0]
     shape = (n, -(-K // group))
-    if scales.dtype not in _TYPES or tuple(scales.shape) != shape:
+    if scales is None or scales.dtype not in _TYPES or tuple(scales.shape) != shape:
         raise ValueError(f"scales: {shape} of fp32, fp16 or bf16 required")
     if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != shape):
         raise ValueError(f"zeros: uint8 {shape} required")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in (x.dtype, torch.float32):
         raise ValueError("out_dtype must be x's type or fp32")
-    _inference("int4_linear", x.device, (x, weight, scales, zeros, bias), _INT4_TENSORS)
     if K > 1 and x.stride(1) != 1 or x.stride(0) < K:
         x = x.contiguous()
     scales = scales.contiguous()

@@ -12,6 +12,8 @@ from __future__ import annotations
 import ctypes
 import math
 
+import torch
+
 from . import ops
 
 MAX_HEAD_DIM = 256
@@ -107,6 +109,8 @@ def packed_qk_norm_rope(qkv, heads: int, kv_heads: int, positions, axes: RotaryA
     """qk_norm_rope in place on packed rows [S, (heads + 2 kv_heads) * D] = [q | k | v] of one
     rank's QKV projection.  Returns the views (q, k, v), each [S, H, D]."""
     D = axes.head_dim
+    if not isinstance(qkv, torch.Tensor):
+        raise ValueError("qkv: tensor required")
     if qkv.ndim != 2 or qkv.shape[1] != (heads + 2 * kv_heads) * D:
         raise ValueError(f"qkv: [S, {(heads + 2 * kv_heads) * D}] required, got {tuple(qkv.shape)}")
     a, b = heads * D, (heads + kv_heads) * D

@@ -175,3 +175,36 @@ def test_outputs_may_not_overlap_what_is_read(cuda_device):
     want, _ = qk_norm_rope(q.clone(), None, pos, axes, q_weight=w.clone())
     qk_norm_rope(q, None, pos, axes, q_weight=w, out_q=q)
     assert torch.equal(q, want)
+
+
+# --------------------------------------------------------------------------------------
+# arguments that are no tensors
+# --------------------------------------------------------------------------------------
+def test_arguments_that_are_no_tensors(cuda_device):
+    from h3tp import ops
+    from h3tp.rms_rope import RotaryAxes, packed_qk_norm_rope, qk_norm_rope
+    x = torch.zeros(2, 64, dtype=torch.float16, device="cuda")
+    w = torch.zeros(16, 32, dtype=torch.uint8, device="cuda")
+    s, z = torch.zeros(16, 2, device="cuda"), torch.zeros(16, 2, dtype=torch.uint8, device="cuda")
+    axes, pos = RotaryAxes(64, (64,)), torch.zeros(2, dtype=torch.int32, device="cuda")
+    q = x.view(2, 1, 64)
+    for bad in (3, [1.0], "x"):
+        for call in (lambda: ops.residual_norm(bad), lambda: ops.residual_norm(x, bad),
+                     lambda: ops.residual_norm(x, x.clone(), bad), lambda: ops.residual_norm(x, x.clone(), out=bad),
+                     lambda: ops.residual_norm(x, x.clone(), labels=bad),
+                     lambda: ops.residual_norm(x, pre=ops.NormSpec("rms", bad)),
+                     lambda: ops.residual_norm(x, pre=ops.NormSpec(), shift=bad),
+                     lambda: ops.int4_linear(bad, w, s, group=32), lambda: ops.int4_linear(x, bad, s, group=32),
+                     lambda: ops.int4_linear(x, w, bad, group=32), lambda: ops.int4_linear(x, w, s, bad, group=32),
+                     lambda: ops.int4_linear(x, w, s, z, group=32, bias=bad),
+                     lambda: qk_norm_rope(bad, None, pos, axes), lambda: qk_norm_rope(q, bad, pos, axes),
+                     lambda: qk_norm_rope(q, None, bad, axes), lambda: qk_norm_rope(q, None, pos, bad),
+                     lambda: qk_norm_rope(q, None, pos, axes, q_weight=bad),
+                     lambda: qk_norm_rope(q, None, pos, axes, out_q=bad),
+                     lambda: packed_qk_norm_rope(bad, 1, 1, pos, axes)):
+            with pytest.raises(ValueError):
+                call()
+    for call in (lambda: ops.int4_linear(x, None, s, group=32), lambda: ops.int4_linear(x, w, None, group=32),
+                 lambda: qk_norm_rope(q, None, pos, None), lambda: qk_norm_rope(q, None, None, axes)):
+        with pytest.raises(ValueError):
+            call()
