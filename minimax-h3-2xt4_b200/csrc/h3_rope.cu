@@ -414,7 +414,11 @@ extern "C" int h3_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, i
       turns == nullptr || axis == nullptr || pairs < 1 || 2 * pairs > head_dim ||
       pos_kind < H3_POS_I32 || pos_kind > H3_POS_F32 || type < H3_TYPE_F32 || type > H3_TYPE_BF16)
     return H3_ERR_INVALID;
+  // a stride that is never taken may be anything: no range or alignment is asked of it
   if (k == nullptr) k_token = k_head = ko_token = ko_head = 0;
+  if (tokens <= 1) q_token = qo_token = k_token = ko_token = 0;
+  if (q_heads == 1) q_head = qo_head = 0;
+  if (k_heads == 1) k_head = ko_head = 0;
   for (int64_t s : {q_token, q_head, qo_token, qo_head, k_token, k_head, ko_token, ko_head})
     if (s < 0 || s > 0x7fffffff) return H3_ERR_INVALID;
   RopeArgs a;

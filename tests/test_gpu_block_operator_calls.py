@@ -208,3 +208,21 @@ def test_arguments_that_are_no_tensors(cuda_device):
                  lambda: qk_norm_rope(q, None, pos, None), lambda: qk_norm_rope(q, None, None, axes)):
         with pytest.raises(ValueError):
             call()
+
+
+# --------------------------------------------------------------------------------------
+# in place through another view of the same heads
+# --------------------------------------------------------------------------------------
+def test_in_place_through_another_view(cuda_device):
+    """The stride of a dimension of one does not make an output another tensor than its input."""
+    from h3tp.rms_rope import RotaryAxes, qk_norm_rope
+    axes, pos = RotaryAxes(64, (64,)), torch.arange(5, device="cuda")
+    x = _randn(1, 5, 64).half()
+    for q, out in ((x.view(5, 1, 64), x.as_strided((5, 1, 64), (64, 7, 1))),
+                   (x.view(1, 5, 64), x.as_strided((1, 5, 64), (9999, 64, 1)))):
+        keep = x.clone()
+        at = pos[:q.shape[0]]
+        want, _ = qk_norm_rope(q.clone(), None, at, axes)
+        got, _ = qk_norm_rope(q, None, at, axes, out_q=out)
+        assert got is out and torch.equal(q, want)
+        x.copy_(keep)
