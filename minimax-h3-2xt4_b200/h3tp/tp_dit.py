@@ -432,7 +432,8 @@ class TPDiTModulatedBlockINT8(nn.Module):
     heads counts the heads of all ranks, head_dim is the plan's; `attention` takes (q, k, v),
     each [S, heads / world, head_dim] fp16 (views of one packed tensor), and returns
     [S, heads / world, head_dim]; without one the values pass through.  Norm weights and the
-    modulation are replicated over the ranks."""
+    modulation are replicated over the ranks.  LoRA adapters on qkv_proj or fc1, whose inputs
+    exist as codes only, are refused."""
 
     def __init__(self, hidden: int, ffn: int, heads: int, axes, cond_features: int, rank: int = 0,
                  world_size: int = 1, device=None, policy=None, comm=None, eps: float = 1e-6,
@@ -470,6 +471,9 @@ class TPDiTModulatedBlockINT8(nn.Module):
         from . import ops
         from .dit_fusion import labels_for
         from .rms_rope import packed_qk_norm_rope
+        for m in (self.qkv_proj, self.fc1):  # before x is changed
+            if getattr(m, "lora_adapter", None) is not None:
+                raise ValueError("no LoRA on qkv_proj or fc1: their inputs exist as codes only")
         labels = None
         if cond.shape[0] != 1:
             labels = labels_for(x, segments, cond.shape[0])

@@ -226,3 +226,33 @@ def test_in_place_through_another_view(cuda_device):
         got, _ = qk_norm_rope(q, None, at, axes, out_q=out)
         assert got is out and torch.equal(q, want)
         x.copy_(keep)
+
+
+# --------------------------------------------------------------------------------------
+# the block
+# --------------------------------------------------------------------------------------
+def _block():
+    from h3tp.rms_rope import RotaryAxes
+    from h3tp.tp_dit import TPDiTModulatedBlockINT8
+    block = TPDiTModulatedBlockINT8(256, 256, 4, RotaryAxes(64, (64,)), 64, device="cuda", group=32)
+    for m in (block.qkv_proj, block.out_proj, block.fc1, block.fc2):
+        m.weight.data.random_(-100, 101)
+        m.weight_scale.data.fill_(1e-4)
+    block.modulation.load_from_full(_randn(1, 6 * 256, 64) * 0.05, _randn(2, 6 * 256))
+    return block
+
+
+class _Adapter:
+    def add_to(self, source, out, **kw):
+        return out
+
+
+@pytest.mark.parametrize("which", ["qkv_proj", "fc1"])
+def test_block_refuses_an_adapter_before_it_changes_the_residual(cuda_device, which):
+    block = _block()
+    getattr(block, which).lora_adapter = _Adapter()
+    x, pos = _randn(3, 40, 256).half(), torch.arange(40, device="cuda")
+    keep = x.clone()
+    with pytest.raises(ValueError):
+        block(x, _randn(4, 1, 64).half(), pos)
+    assert torch.equal(x, keep)
