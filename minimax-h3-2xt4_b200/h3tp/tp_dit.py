@@ -444,6 +444,15 @@ class TPDiTModulatedBlockINT8(nn.Module):
         inner = heads * axes.head_dim
         if heads % world_size or hidden % 256 or (inner // world_size) % 256:
             raise ValueError("heads must divide by the ranks; hidden and a rank's heads * head_dim by 256")
+        policy = policy or H3OperatorPolicy(fc1_swiglu_epilogue=True)
+        if ffn < 1 or ffn % world_size or ffn % 256:
+            raise ValueError("ffn must divide by the ranks and by 256")
+        # the FP32 activation of FC1's epilogue goes through the fused FC2 route alone
+        if policy.fc1_swiglu_epilogue and (ffn // world_size % 256 or world_size not in (1, 2, 4, 8)
+                                           or policy.fc2_quantizer not in ("fused_stored", "fused_recompute")
+                                           or policy.row_linear_backend == "native"):
+            raise ValueError("fc1_swiglu_epilogue needs 256 columns of ffn to a rank, or a multiple, and the "
+                             "fused FC2 quantiser")
         # one device for the sharded projections and for what every rank holds whole
         device = torch.device(device) if device is not None else torch.device("cuda", rank)
         self.hidden, self.heads, self.axes, self.eps = hidden, heads // world_size, axes, eps
@@ -461,7 +470,7 @@ class TPDiTModulatedBlockINT8(nn.Module):
         self.attn_norm, self.attn_post_norm = ones(hidden), ones(hidden)
         self.mlp_norm, self.mlp_post_norm = ones(hidden), ones(hidden)
         self.q_norm, self.k_norm = ones(axes.head_dim), ones(axes.head_dim)
-        configure_block(self, "dit", policy or H3OperatorPolicy(fc1_swiglu_epilogue=True))
+        configure_block(self, "dit", policy)
 
     def forward(self, x: torch.Tensor, cond: torch.Tensor, positions: torch.Tensor, attention=None,
                 segments=None) -> torch.Tensor:

@@ -144,3 +144,31 @@ def test_two_ranks_agree_with_one(tmp_path):
     assert np.array_equal(got[2][0], got[2][1])
     one, two = got[1][0], got[2][0]
     assert np.linalg.norm(two - one) <= 4 * 0.009 * np.linalg.norm(one)
+
+
+# --------------------------------------------------------------------------------------
+# shapes and policies that the second half of a forward could not run
+# --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("ffn,world,policy", [
+    (640, 1, {}), (1280, 2, {}), (1023, 2, {}), (0, 1, {}), (1024, 1, {"fc2_quantizer": "native"}),
+    (1024, 1, {"fc2_quantizer": "owned_fp32"}), (1024, 1, {"row_linear_backend": "native"}),
+    (640, 1, {"fc1_swiglu_epilogue": False})])
+def test_block_refuses_what_fc2_cannot_take(ffn, world, policy):
+    """Refused when the block is made, not after a forward has changed the residual."""
+    from h3tp.h3_operator_policy import H3OperatorPolicy
+    from h3tp.rms_rope import RotaryAxes
+    from h3tp.tp_dit import TPDiTModulatedBlockINT8
+    policy = H3OperatorPolicy(**{"fc1_swiglu_epilogue": True, **policy})
+    with pytest.raises(ValueError):
+        TPDiTModulatedBlockINT8(512, ffn, 8, RotaryAxes(64, (64,)), 64, 0, world, device="cpu", policy=policy)
+
+
+@pytest.mark.parametrize("ffn,world,policy", [
+    (1024, 2, {}), (1280, 2, {"fc1_swiglu_epilogue": False}),
+    (1024, 1, {"fc1_swiglu_epilogue": False, "fc2_quantizer": "native"})])
+def test_block_takes_what_fc2_takes(ffn, world, policy):
+    from h3tp.h3_operator_policy import H3OperatorPolicy
+    from h3tp.rms_rope import RotaryAxes
+    from h3tp.tp_dit import TPDiTModulatedBlockINT8
+    policy = H3OperatorPolicy(**{"fc1_swiglu_epilogue": True, **policy})
+    TPDiTModulatedBlockINT8(512, ffn, 8, RotaryAxes(64, (64,)), 64, 0, world, device="cpu", policy=policy)
