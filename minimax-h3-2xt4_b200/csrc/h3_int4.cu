@@ -2,15 +2,14 @@
 //   y[m][n] = sum_g scale[n][g] * sum_{k in g} x[m][k] (code[n][k] - zero[n][g]) + bias[n]
 // code k of a row is the low nibble of byte k / 2 for even k, the high one for odd k.
 //
-// Bound by the weight's bytes: each is read once.  What stands between that and a plain
+// The floor is the weight's bytes, each read once.  What stands between that and a plain
 // product is the unpacking (one weight in half a byte) and, for more than a row or two, the
 // multiplications.  Both go to where they cost least: a warp takes 16 output columns and
 // runs m16n8k16 products with the unpacked weights as the 16-row operand and eight rows of
-// x as the other, so a weight is unpacked once for eight rows, two at a time, exactly
-// (code - zero is a small integer in either 16-bit type), and the group's scale is applied
-// to the fp32 sum of the group.  (The fifth-generation tensor cores would want the unpacked
-// weights in shared memory, four times the bytes of the packed ones; at so few rows the
-// older instruction is far from its limit.)
+// x as the other, so a weight is unpacked once for the CTA's rows (8, 16 or 32), two at a
+// time, exactly (code - zero is a small integer in either 16-bit type), and the group's scale
+// is applied to the fp32 sum of the group.  (tcgen05.mma could take the unpacked weights from tensor memory,
+// written there by tcgen05.st; that form has not been built.)
 //
 // The order of k inside a product does not matter as long as both operands agree and a
 // product stays inside a group, so the weights need no layout of their own: lane t of a row's
@@ -20,10 +19,12 @@
 // loaded straight into registers, as far ahead as those allow, the same products took 44 us
 // against 38 (9 x 5376 x 32256, fp16, groups of 128).
 //
-// That case reads 92 MB, 14 us at the measured copy rate; the kernel needs 38 us (0.38), a
-// single row of 5120 x 25600 in groups of 64 with zeros 28 us (0.39): bound by the issue of
-// about 50 instructions for 16 x 32 weights, 18 of them the unpacking, with the logical ones
-// at half rate.
+// That case reads 92 MB, 14 us at the measured copy rate; the kernel needs 38 us (0.37), a
+// single row of 5120 x 25600 in groups of 64 with zeros 29 us (0.38).  No unit is at its limit:
+// of the issue slots 50% and 62% are busy, of the ALU 37% and 53%, of the tensor pipe 29% and
+// 14%.  One CTA of 14 and 11 working warps an SM (128 registers a thread, the ring) leaves
+// too few warps to cover the waits for weights, for fixed latencies and for the math pipe
+// between the 51 and 64 instructions for 16 x 32 weights, 18 of them the unpacking.
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -67,7 +68,9 @@ struct Unpack;
 // Eight codes of a word as four pairs (code i, code i + 4) of exact integers code - zero.
 // A 16-bit float whose mantissa's low bits are the code is a power of two plus the code:
 // 1024 + c in fp16 (or 1024 + 16 c for the upper nibble, scaled back in the subtraction) and
-// 128 + c in bf16, so one logical operation and one exact fma unpack two codes.
+// 128 + c in bf16, so one logical operation and one exact fma unpack two codes.  (The method of
+// Y. J. Kim, R. Henry, R. Fahim and H. Awadalla, "Who Says Elephants Can't Run: Bringing Large
+// Scale MoE Models into Cloud Scale Production", 2022; the constants follow from the formats.)
 template <>
 struct Unpack<__half> {
   uint32_t low, high;  // -(1024 + zero) and -(64 + zero) in both halves
@@ -427,8 +430,9 @@ int launch_int4(Int4Args& a, int dev, cudaStream_t stream) {
   auto kern = int4_kernel<T, S, ZEROS, MT, GB, VEC>;
   // Column tiles at a time.  The busiest SM's time in stages: its warps' work, which about 12
   // warps saturate, or the longest chain of one warp; and for each round the joining of the
-  // slices (1 x 5120 x 25600: 28 us as 12 tiles without slices, 33 as 4 tiles of 4 slices
-  // in 3 rounds, 44 as 1 of 16 in 11).
+  // slices (1 x 5120 x 25600: 28.4 us as 11 tiles without slices, which the rule takes, 28.7 as
+  // 12, 34.8 as 16, 31.7 as 4 tiles of 4 slices in 3 rounds, 52.5 as 8 of 2 in 2, 44.0 as 1 of
+  // 16 in 11; 9 x 5376 x 32256: 38.0 as 14, 38.7 as 16, 47.6 as 4, 45.3 as 8, 85.2 as 12 in 2).
   const int stages = (a.k + kStageK - 1) / kStageK, tiles = (a.n + 15) / 16;
   const int blocks_m = (int)((a.m + 8 * MT - 1) / (8 * MT));
   const int ctas = std::max(1, h3host::sm_count(dev) / blocks_m);
@@ -464,8 +468,10 @@ int launch_int4_shape(Int4Args& a, int dev, cudaStream_t stream) {
   const bool vec = a.k % 32 == 0 && h3host::aligned(a.w, 16);
   if (a.m <= 8) return vec ? launch_int4<T, S, ZEROS, 1, GB, true>(a, dev, stream)
                            : launch_int4<T, S, ZEROS, 1, GB, false>(a, dev, stream);
-  // 16 rows a CTA, or 32 where all of their x fits (32 x 12800 x 5120: 63 us as two blocks
-  // of 16 rows, 88 as one of 32 with two and a half times the chunks of x)
+  // 16 rows a CTA, or 32 where all of their x fits (32 x 12800 x 5120: 60 us as two blocks
+  // of 16 rows, 88 as one of 32 with two and a half times the chunks of x).  The border is
+  // rough: 32 x 1152 x 12800 takes 17 us as one block and would take 14 as two, 17 rows of
+  // 5120 x 25600 take 87 as two and would take 66 as one, of 2816 x 25600 44 as two and 38 as one.
   const int64_t rows = std::min<int64_t>(a.m, 32), x32 = (rows + 1) * (2 * (int64_t)a.k + 512 + 64);
   if (a.m <= 16 || x32 + kInt4Warps * (kStages * 16 * (vec ? kSlotRow<true> : kSlotRow<false>) + rows * 64) > kInt4Smem)
     return vec ? launch_int4<T, S, ZEROS, 2, GB, true>(a, dev, stream)

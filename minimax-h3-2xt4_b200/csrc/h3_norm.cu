@@ -7,16 +7,17 @@
 // in fp32 between the two roundings.
 //
 // Bound by HBM: x and the branch are read once, x' and h (or the codes) written once; the
-// row lives in registers from its load to its last store, eight values a thread, one CTA a
-// row.  What else a row needs is kept off the memory's path: the modulation tables and the
+// row lives in registers from its load to its last store: eight values a thread, one or two
+// rows a CTA at a time, and in rows wider than 8192 values 32 a thread.  What else a row needs is kept off the memory's path: the modulation tables and the
 // norms' weights, four times the row's own bytes, are folded into three factors a value
 // and stay in registers until a row has another label, and rows to come are fetched by
 // cp.async into slots of shared memory that only the fetching thread reads.
 //
-// 32768 x 3072 fp16 with both norms, gate and h stored (805 MB): 178 us, 0.69 of the measured
-// copy rate; with codes of the rotated row instead of h (705 MB) 245 us, 0.44, the rotation's
-// shuffles and the quantiser filling the issue slots.  One row at a time and factors read
-// from memory, the second took 376 us.
+// 32768 x 3072 fp16 with both norms, gate and h stored (805 MB): 175 us, 0.70 of the measured
+// copy rate; with codes of the rotated row instead of h (705 MB) 241 us, 0.45.  Neither is at a
+// unit's limit: 49% and 61% of the issue slots are busy at 37% occupancy, and warps wait for
+// the next rows, the barriers and the shuffles.  One row at a time and factors read from
+// memory, the second took 376 us.
 #include "h3_types.cuh"
 
 namespace h3 {
@@ -381,7 +382,8 @@ H3_DEV void quantise(f32x2 (&v)[ROWS][NC][4], const ResidualNorm& a, const Deal&
       if (finite[r]) {
         // the correctly rounded quotient (div_by_scale's correction of v * inv), as the library's
         // other quantisers take it: v * inv alone falls to the other side of a border between
-        // codes once in about two million values (32768 x 3072 fp16: 244 us with it alone, 250 so).
+        // codes once in about two million values (32768 x 3072 fp16, calls one after the other: 244 us
+        // with it alone, 250 so).
         // |v| / scale <= 127 (1 + 2^-23), so no code leaves the range, and the sum with
         // 1.5 * 2^23 rounds to the nearest integer, ties to even, in the low byte
         const f32x2 i2 = dup2(inv), ns = dup2(-scale);

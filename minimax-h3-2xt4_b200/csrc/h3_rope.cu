@@ -7,19 +7,20 @@
 // the token and the pair alone, so a lane group takes one token and walks over its heads
 // with the angles, times the norm's weights, in registers: no barrier anywhere.  A head is
 // held by G = 8, 16 or 32 lanes, eight elements (four pairs) each; the sum of squares is a
-// shuffle tree over those lanes.  Each lane keeps up to 64 bytes of the heads to come in flight
-// through cp.async into slots of shared memory that it alone reads: held in registers,
-// the same bytes left too few warps an SM to cover the memory's latency (158 against
+// shuffle tree over those lanes.  Each lane keeps the heads to come in flight (three steps, 48
+// bytes, of a 16-bit type; one step, 32 bytes, of fp32) through cp.async into slots of shared
+// memory that it alone reads: held in registers, the same bytes left too few warps an SM to cover the memory's latency (158 against
 // 143 us).  32768 tokens of 24 + 24 heads of 128 in fp16, 805 MB: 140 us, 5.7 TB/s, 0.88 of
-// the measured copy rate (halves paired: 156 us).
+// the measured copy rate (halves paired: 156 us; 12 + 12 heads in fp32, the same bytes: 201 us,
+// halves 143).  Heads of 72, 80 and 96 take the 16 lanes of 128 and its 141 us.
 #include "h3_types.cuh"
 
 namespace h3 {
 
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 constexpr int kRopeThreads = 256;
-// Four CTAs an SM (64 registers a thread) and 64 bytes a lane in flight; three, five or six
-// CTAs and 128 bytes measured up to 10% slower at 32768 tokens of 48 heads.
+// Four CTAs an SM (64 registers a thread) and slots of 64 bytes a lane, one of them being
+// used up; three, five or six CTAs and 128 bytes measured up to 10% slower at 32768 tokens of 48 heads.
 constexpr int kRopeCtas = 4;
 constexpr int kRopeSlotBytes = 64;
 
