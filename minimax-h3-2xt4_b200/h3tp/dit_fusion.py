@@ -48,15 +48,18 @@ class _LabelCache:
     waited for before it is cached, so it is complete for every stream that reads it
     later; a reader on a stream other than the one that built it is recorded on the
     tensor, so the allocator keeps the memory until that stream's work is done even if
-    the entry is evicted meanwhile."""
+    the entry is evicted meanwhile.  A graph that captures a reader replays with the
+    tensor's address long after: a vector read under capture is kept for good."""
 
     def __init__(self, capacity: int = 8):
         self.capacity = capacity
         self.tables: dict = {}
+        self.captured: dict = {}
 
     def get(self, device: torch.device, rows: int, key: tuple) -> torch.Tensor:
         table = self.tables.setdefault(device, OrderedDict())
-        entry = table.get((rows, key))
+        kept = self.captured.get((device, rows, key))
+        entry = kept or table.get((rows, key))
         if entry is None:
             ordered = sorted(key)
             labels = np.repeat(np.array([t[2] for t in ordered], dtype=np.int32),
@@ -69,12 +72,14 @@ class _LabelCache:
             table[(rows, key)] = entry
             while len(table) > self.capacity:
                 table.popitem(last=False)
-        else:
+        elif kept is None:
             table.move_to_end((rows, key))
         tensor, built_on = entry
         reader = torch.cuda.current_stream(device)
         if reader != built_on:
             tensor.record_stream(reader)
+        if kept is None and torch.cuda.is_current_stream_capturing():
+            self.captured[device, rows, key] = table.pop((rows, key))
         return tensor
 
 

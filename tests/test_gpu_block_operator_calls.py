@@ -256,3 +256,37 @@ def test_block_refuses_an_adapter_before_it_changes_the_residual(cuda_device, wh
     with pytest.raises(ValueError):
         block(x, _randn(4, 1, 64).half(), pos)
     assert torch.equal(x, keep)
+
+
+def test_captured_block_keeps_its_labels(cuda_device):
+    """The labels of captured calls stay as they are, however many other segment layouts come
+    between captures and replays."""
+    from h3tp.dit_fusion import labels_for
+    block = _block()
+    x0, cond, pos = _randn(5, 640, 256).half(), _randn(6, 2, 64).half(), torch.arange(640, device="cuda")
+    segments = [(0, 77, 0), (77, 640, 1)]
+    want = x0.clone()
+    block(want, cond, pos, segments=segments)
+
+    def other_layouts():
+        for i in range(16):
+            labels_for(x0, [(0, 100 + i, 1), (100 + i, 640, 0)], 2)
+        torch.cuda.synchronize()
+        return [torch.zeros(640, dtype=torch.int32, device="cuda") for _ in range(64)]
+
+    runs, others = [], []
+    for _ in range(2):
+        x = x0.clone()
+        block(x, cond, pos, segments=segments)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            block(x, cond, pos, segments=segments)
+        runs.append((x, graph))
+        others += other_layouts()
+    for x, graph in runs:
+        x.copy_(x0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, want)
+    assert all(int(t.sum()) == 0 for t in others)
