@@ -290,3 +290,56 @@ def test_captured_block_keeps_its_labels(cuda_device):
         torch.cuda.synchronize()
         assert torch.equal(x, want)
     assert all(int(t.sum()) == 0 for t in others)
+
+
+# --------------------------------------------------------------------------------------
+# offsets past 32 bits
+# --------------------------------------------------------------------------------------
+def test_offsets_past_32_bits(cuda_device):
+    """The last rows, tokens and columns of tensors of more than 2^31 elements (of int4_linear's
+    weight: bytes) come out as in small calls."""
+    from h3tp import ops
+    from h3tp.rms_rope import RotaryAxes, qk_norm_rope
+    rows, width = 690003, 3200
+    x = torch.ones(rows, width, dtype=torch.float16, device="cuda")
+    b = torch.ones_like(x)
+    x[-9:], b[-9:] = _randn(1, 9, width), _randn(2, 9, width)
+    kw = dict(pre=ops.NormSpec(), quantize=True, convrot=False)
+    want = ops.residual_norm(x[-9:].clone(), b[-9:].clone(), **kw)
+    got = ops.residual_norm(x, b, **kw)
+    assert all(torch.equal(g[-9:], w) for g, w in zip(got, want))
+    del x, b, got
+
+    tokens, stride = 54001, 40000
+    packed = torch.empty(tokens, stride, dtype=torch.float16, device="cuda")
+    packed[:, -256:] = _randn(3, tokens, 256)
+    q, k = (packed[:, a:a + 128 or None].unflatten(1, (2, 64)) for a in (-256, -128))
+    axes, pos = RotaryAxes(64, (32, 32)), torch.randint(0, 9999, (tokens, 2), device="cuda")
+    want = qk_norm_rope(q.contiguous(), k.contiguous(), pos, axes)
+    got = qk_norm_rope(q, k, pos, axes, out_q=q, out_k=k)
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    del packed, q, k, got, want
+
+    # x, codes and scales are small integers: every sum is exact, in any order
+    n, k = 270000, 16384
+    w = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda")
+    s = torch.randint(1, 4, (n, k // 128), device="cuda").float()
+    x = torch.randint(-2, 3, (3, k), device="cuda").half()
+    y = ops.int4_linear(x, w, s, out_dtype=torch.float32)
+    assert torch.equal(y[:, -40:], ops.int4_linear(x, w[-40:].contiguous(), s[-40:], out_dtype=torch.float32))
+    del w, s, y
+    m, n = 40000, 54000
+    w = torch.randint(0, 256, (n, 16), dtype=torch.uint8, device="cuda")
+    s, x = torch.ones(n, 1, device="cuda"), torch.randint(-2, 3, (m, 32), device="cuda").half()
+    y = ops.int4_linear(x, w, s, group=32)
+    assert torch.equal(y[-17:], ops.int4_linear(x[-17:], w, s, group=32))
+
+
+def test_int4_linear_most_rows(cuda_device):
+    from h3tp import ops
+    w = torch.randint(0, 256, (16, 16), dtype=torch.uint8, device="cuda")
+    s, x = torch.ones(16, 1, device="cuda"), torch.randint(-2, 3, (16 * 65535 + 1, 32), device="cuda").half()
+    y = ops.int4_linear(x[:-1], w, s, group=32)
+    assert torch.equal(y[-21:], ops.int4_linear(x[-22:-1], w, s, group=32))
+    with pytest.raises(ValueError):
+        ops.int4_linear(x, w, s, group=32)
