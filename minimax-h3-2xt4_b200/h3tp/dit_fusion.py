@@ -10,6 +10,7 @@ the reference (tilelang_dit_fusion.py:153-168).
 """
 from __future__ import annotations
 
+import threading
 from collections import OrderedDict
 
 import numpy as np
@@ -49,14 +50,20 @@ class _LabelCache:
     later; a reader on a stream other than the one that built it is recorded on the
     tensor, so the allocator keeps the memory until that stream's work is done even if
     the entry is evicted meanwhile.  A graph that captures a reader replays with the
-    tensor's address long after: a vector read under capture is kept for good."""
+    tensor's address long after: a vector read under capture is kept for good.  Calls on
+    several threads look up and build one after the other."""
 
     def __init__(self, capacity: int = 8):
         self.capacity = capacity
         self.tables: dict = {}
         self.captured: dict = {}
+        self.lock = threading.Lock()
 
     def get(self, device: torch.device, rows: int, key: tuple) -> torch.Tensor:
+        with self.lock:
+            return self._get(device, rows, key)
+
+    def _get(self, device: torch.device, rows: int, key: tuple) -> torch.Tensor:
         table = self.tables.setdefault(device, OrderedDict())
         kept = self.captured.get((device, rows, key))
         entry = kept or table.get((rows, key))

@@ -776,7 +776,8 @@ def int4_linear(x, weight, scales, zeros=None, *, group: int = 128, bias=None, o
     lie between 0 and 15: the call does not read them on the host and larger ones give wrong
     products (ColumnParallelLinearINT4's loader refuses them).
     Meant for few rows (a token or a handful): the weight is read and unpacked once for every 16
-    rows, or for every 32 where their x fits an SM's shared memory (K up to about 1200 for 32 rows, 2900 for 17)."""
+    rows, or for every 32 where their x fits an SM's shared memory (K up to about 1200 for 32
+    rows, 2900 for 17)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.ndim != 2 \
             or x.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError("x: 2-D CUDA tensor of fp16 or bf16 required")

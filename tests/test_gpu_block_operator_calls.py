@@ -343,3 +343,56 @@ def test_int4_linear_most_rows(cuda_device):
     assert torch.equal(y[-21:], ops.int4_linear(x[-22:-1], w, s, group=32))
     with pytest.raises(ValueError):
         ops.int4_linear(x, w, s, group=32)
+
+
+def test_labels_on_several_threads(cuda_device):
+    """More layouts than the table holds, from threads that evict each other's."""
+    from h3tp.dit_fusion import labels_for
+    x = torch.empty(64, 8, device="cuda")
+    wrong = []
+
+    def work(i):
+        try:
+            for k in range(400):
+                cut = 1 + (7 * k + 3 * i) % 62
+                got = labels_for(x, [(0, cut, 1), (cut, 64, 0)], 2)
+                if int(got.sum()) != cut:
+                    wrong.append((i, k))
+        except Exception as e:  # noqa: BLE001 - told below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
+
+
+def test_first_calls_in_a_capture(cuda_device):
+    """A process whose first calls, of sizes that raise the shared-memory limit, are captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from h3tp import ops
+from h3tp.rms_rope import RotaryAxes, qk_norm_rope
+x, b = torch.randn(5, 2944, device="cuda"), torch.randn(5, 2944, device="cuda")
+a, w = torch.randn(3, 256, device="cuda").half(), torch.randint(0, 256, (32, 128), device="cuda", dtype=torch.uint8)
+s, q, pos = torch.ones(32, 2, device="cuda"), torch.randn(4, 2, 64, device="cuda"), torch.arange(4, device="cuda")
+def calls():
+    return (ops.residual_norm(x, b, pre=ops.NormSpec(), out=torch.empty_like(x))[1], ops.int4_linear(a, w, s),
+            qk_norm_rope(q, None, pos, RotaryAxes(64, (64,)))[0])
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    held = calls()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(h, c) for h, c in zip(held, calls()))
+"""
+    pkg = Path(__file__).resolve().parents[1] / "minimax-h3-2xt4_b200"
+    r = subprocess.run([sys.executable, "-c", code, str(pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
