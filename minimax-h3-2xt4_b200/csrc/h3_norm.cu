@@ -645,13 +645,19 @@ int launch_ring(const ResidualNorm& a, const Deal& d, int threads, int dev, cuda
 template <typename XT, typename BT, bool BRANCH, bool QUANT>
 int launch_norm_shape(const ResidualNorm& a, bool vec, int dev, cudaStream_t stream) {
   const int width = (int)a.width;
+  // 1024 threads of eight values are the most; beyond, 32 a thread.  8192 rows bf16 with eight and
+  // with 32: 5376 wide 106 and 121 us, 8192 wide 159 and 156 (but 4096 wide 93 and 81).
   const int nc = width <= 8192 ? 1 : 4;
   const int threads = ((width + 8 * nc - 1) / (8 * nc) + 31) / 32 * 32;
   Deal d{width, 8, 1, 8 * threads};
   if (width % 8 != 0) d = Deal{width, 1, threads, 8 * threads};
   if (nc == 1 && vec) {
     // Two rows at a time where the registers allow it, there are rows for every SM to have
-    // several pairs, and three slots of a pair fit; else one row, in four slots or two.
+    // several pairs, and three slots of a pair fit: fp16 codes, 32768 x 3072 240 us against 295 one
+    // at a time in four slots and 291 in two, 1184 x 3072 18.7 against 20.0 and 19.5, at the border
+    // 592 x 3072 12.0 against 11.8 and 11.5 (narrow rows lose there: 592 x 1024 9.0 against 6.1).
+    // Else one row, in four slots or two, between which little lies (6144 wide, FP32 branch: 346
+    // and 344; but 16384 x 4096 fp32 309 and 265).
     const int64_t pair = 2ll * threads * 8 * (sizeof(XT) + (BRANCH ? sizeof(BT) : 0));
     if (threads <= kPairThreads && a.rows >= 4ll * h3host::sm_count(dev) && 3 * pair <= kRingSmem)
       return launch_ring<XT, BT, BRANCH, QUANT, 2, 3>(a, d, threads, dev, stream);
